@@ -31,7 +31,9 @@ CAPI_SYMBOLS = (
 )
 LFM_SYMBOLS = (
     "lfm_gemm_nt", "lfm_embed", "lfm_rmsnorm", "lfm_qk_norm_rope", "lfm_attention",
-    "lfm_shortconv", "lfm_rope_tables", "lfm_synth_normal", "lfm_fill", "lfm_synth_stream_of",
+    "lfm_shortconv", "lfm_kv_write", "lfm_kv_read", "lfm_kv_attention",
+    "lfm_kv_attention_workspace", "lfm_softmax", "lfm_softmax_workspace", "lfm_verify_draft",
+    "lfm_verify_draft_workspace", "lfm_rope_tables", "lfm_synth_normal", "lfm_fill", "lfm_synth_stream_of",
     "lfm_synth_is_norm", "lfm_synth_tensor", "lfm_model_create_synthetic",
     "lfm_model_create_from_file", "lfm_model_destroy", "lfm_model_forward", "lfm_model_embed",
     "lfm_model_layer_forward", "lfm_model_head", "lfm_model_moe", "lfm_model_info",
@@ -55,6 +57,21 @@ class LfmModelConfig(ctypes.Structure):
                 ("num_dense_layers", ctypes.c_int), ("max_batch", ctypes.c_int),
                 ("max_seq", ctypes.c_int), ("seed", ctypes.c_uint64),
                 ("weight_std", ctypes.c_float)]
+
+
+class LfmKvCache(ctypes.Structure):
+    _fields_ = [("format", ctypes.c_int), ("kv_heads", ctypes.c_int),
+                ("page_tokens", ctypes.c_int), ("num_pages", ctypes.c_int),
+                ("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
+                ("k_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p)]
+
+
+class LfmKvBatch(ctypes.Structure):
+    _fields_ = [("batch", ctypes.c_int), ("tokens", ctypes.c_int), ("max_new", ctypes.c_int),
+                ("max_len", ctypes.c_int), ("new_start", ctypes.c_void_p),
+                ("own_len", ctypes.c_void_p), ("pages", ctypes.c_void_p),
+                ("max_pages", ctypes.c_int), ("prefix_pages", ctypes.c_void_p),
+                ("prefix_len", ctypes.c_int)]
 
 
 class MoeError(RuntimeError):
@@ -120,6 +137,14 @@ def lib() -> ctypes.CDLL:
     L.lfm_qk_norm_rope.argtypes = [_vp, _i, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp]
     L.lfm_attention.argtypes = [_vp, _i, _vp, _i, _i, _i, _i, _i, _i, _vp]
     L.lfm_shortconv.argtypes = [_vp, _vp, _vp, _i, _i, _i, _i, _vp]
+    L.lfm_kv_write.argtypes = [_vp, _vp, _vp, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _i, _vp, _vp]
+    L.lfm_kv_read.argtypes = [_vp, _vp, _vp, _vp, _i, _i, _vp, _vp]
+    L.lfm_kv_attention.argtypes = [_vp, _vp, _vp, _i, _vp, _i, _i, _vp, _sz, _vp, _vp]
+    L.lfm_kv_attention_workspace.argtypes = [_vp, _vp, _i, ctypes.POINTER(_sz)]
+    L.lfm_softmax.argtypes = [_vp, _ll, _vp, _ll, _i, _i, _f, _vp, _sz, _vp]
+    L.lfm_softmax_workspace.argtypes = [_i, _i, ctypes.POINTER(_sz)]
+    L.lfm_verify_draft.argtypes = [_vp] * 6 + [_i, _i, _i, _vp, _vp, _vp, _sz, _vp]
+    L.lfm_verify_draft_workspace.argtypes = [_i, _i, ctypes.POINTER(_sz)]
     L.lfm_rope_tables.argtypes = [_vp, _vp, _i, _i, _f]
     L.lfm_synth_normal.argtypes = [_vp, _sz, _u64, _u64, _f, _u64, _vp]
     L.lfm_fill.argtypes = [_vp, _sz, _f, _vp]

@@ -42,6 +42,50 @@ hipError_t launch_attention(const float *qkv, int ld, float *out, int batch, int
 hipError_t launch_shortconv(const float *bcg, const float *w, float *y, int batch, int seq,
                             int H, int L, hipStream_t st);
 
+// A call on the paged KV cache (include/lfm_capi.h: lfm_kv_cache, lfm_kv_batch),
+// by value to the kernels.  page_tokens = 1 << pshift.
+struct KvArgs {
+  char *k, *v;
+  float *ks, *vs;
+  const int *new_start, *own_len, *pages, *prefix_pages;
+  int *bad;
+  int format, kv_heads, pshift, num_pages;
+  int batch, tokens, max_new, max_len, max_pages, prefix_len;
+};
+
+// Rows of the new tokens into the cache; with q_weight not null q and k are
+// normalised and rotated first (q in place).
+struct KvWriteArgs {
+  float *qkv;
+  const float *q_weight, *k_weight, *cos_t, *sin_t;
+  int ld, heads, k_col, v_col, max_pos;
+};
+hipError_t launch_kv_write(const KvArgs &a, const KvWriteArgs &w, hipStream_t st);
+
+// Own positions p < rows of sequence b to row b*rows + p of k_out / v_out [..][ld].
+hipError_t launch_kv_read(const KvArgs &a, float *k_out, float *v_out, int rows, int ld,
+                          hipStream_t st);
+
+// Attention of the new tokens over the cache; ws of kv_attention_ws bytes.
+size_t kv_attention_ws(const KvArgs &a, int heads);
+hipError_t launch_kv_attention(const KvArgs &a, const float *q, int ld, float *out, int ldo,
+                               int heads, void *ws, hipStream_t st);
+
+size_t softmax_ws(int rows, int dim);
+hipError_t launch_softmax(const float *x, long long xs, float *y, long long ys, int rows, int dim,
+                          float temperature, void *ws, hipStream_t st);
+
+struct VerifyArgs {
+  const float *target, *draft;
+  const int *ids;
+  const float *u_accept, *u_sample;
+  const int *n_valid;
+  int *accepted, *tokens;
+  int batch, n_draft, vocab;
+};
+size_t verify_draft_ws(int batch, int vocab);
+hipError_t launch_verify_draft(const VerifyArgs &a, void *ws, hipStream_t st);
+
 // dst[i] = sd * N(0,1) sample (first + i) of (seed, stream), the generator of
 // include/moe_synth.h evaluated on the device.
 hipError_t launch_synth_normal(float *dst, size_t n, uint64_t seed, uint64_t stream, float sd,

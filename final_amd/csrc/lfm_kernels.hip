@@ -23,6 +23,7 @@
 #include <algorithm>
 
 #include "gpu_common.h"
+#include "lfm_rope.h"
 #include "skinny_tile.h"
 #include "split_tile.h"
 
@@ -188,18 +189,8 @@ constexpr int kHeadDim = 64;
 // One wave per token (or part of it): its heads + kv_heads rows of 64 (q heads at columns
 // h*64, k heads at k_col + h*64), four rows per float4 load (16 lanes per
 // row, lane l holding elements 4(l%16)..4(l%16)+3), with the cos/sin row of
-// the token's position and both norm weights held in registers.  The norm is
-// rms_norm_kernel on a 64-wide row launched with 256 threads (layer.cu:1146):
-// threads 0..63 hold one square each (fmaf(x, x, 0) = x*x), warps 0 and 1
-// fold elements 0..31 and 32..63 with shuffle-down at 16..1, and the 8-warp
-// fold adds warps 2..7's zeros, which leaves warp0 + warp1.  The same binary
-// tree runs here over the float4 layout (16 -> 4 lanes down, 8 -> 2 lanes,
-// 4 -> 1 lane, then 2 and 1 across a lane's components), so every addition is
-// the reference's.  Then rope_transpose_kernel's rotation (layer.cu:217-228)
-// for position s = t % seq: out[d] = q1*c1 - q2*s1, out[d+32] = q2*c2 + q1*s2
-// with q1 = x[d], q2 = x[d+32] (element d + 32 is 8 lanes up); nvcc's
-// contraction of each line is restated as fmaf(first product, -/+ second
-// product).
+// the token's position s = t % seq and both norm weights held in registers; the
+// arithmetic is norm_rope_row's.
 constexpr int kRopeTokens = 4;   // tokens per block, one per wave
 constexpr int kRopeGroups = 16;  // groups of 4 rows of a token: heads + kv_heads <= 64
 // Up to kRopeSplitTokens a wave takes NG = 4 of a token's groups, grid.y the
@@ -241,29 +232,7 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(float *qkv, int ld, c
   for (int j = 0; j < NG; ++j) {
     if (j >= ng) continue;  // wave-uniform
     const int row = 4 * (g0 + j) + r;
-    f32x4 sq;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) sq[i] = x[j][i] * x[j][i];
-    f32x4 a, b, cc;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) a[i] = sq[i] + __shfl_down(sq[i], 4, 16);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) b[i] = a[i] + __shfl_down(a[i], 2, 16);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) cc[i] = b[i] + __shfl_down(b[i], 1, 16);
-    const float f = (cc[0] + cc[2]) + (cc[1] + cc[3]);
-    const float total = __shfl(f, 16 * r) + __shfl(f, 16 * r + 8);
-    const float rms = 1.0f / sqrtf(total / (float)kHeadDim + moe::kNormEps);
-    const f32x4 w = row < heads ? wq : wk;
-    f32x4 y, other, o;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) y[i] = (x[j][i] * rms) * w[i];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) other[i] = __shfl_xor(y[i], 8);
-    const bool lo = (lane & 15) < 8;  // elements d < 32
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      o[i] = lo ? __builtin_fmaf(y[i], cs[i], -(other[i] * sn[i])) : __builtin_fmaf(y[i], cs[i], other[i] * sn[i]);
+    const f32x4 o = norm_rope_row(x[j], row < heads ? wq : wk, cs, sn);
     if (row < per_tok) __builtin_amdgcn_raw_buffer_store_b128(o, rs, off[j], 0, 0);
   }
 }

@@ -65,6 +65,98 @@ def shortconv(bcg, conv_w, y, batch, seq, hidden, kernel=CONV_L, stream=None):
                                     _stream(stream)), "lfm_shortconv")
 
 
+# -- serving: the paged KV cache, and sampling ---------------------------------
+
+KV_F32, KV_BF16, KV_INT8, KV_FP8 = 0, 1, 2, 3
+
+
+class KVCache:
+    """The caller's cache buffers (lfm_kv_cache): k and v [num_pages][kv_heads][page_tokens][64]
+    of the format's type, and fp32 scales [num_pages][kv_heads][page_tokens] for int8 and fp8.
+    Holds addresses, no memory."""
+
+    def __init__(self, fmt: int, num_pages: int, page_tokens: int, k, v, k_scale=None,
+                 v_scale=None, kv_heads: int = KV_HEADS):
+        self._keep = (k, v, k_scale, v_scale)
+        self.c = _native.LfmKvCache(fmt, kv_heads, page_tokens, num_pages, _ptr(k), _ptr(v),
+                                    _ptr(k_scale), _ptr(v_scale))
+        self.ref = ctypes.byref(self.c)
+
+
+class KVBatch:
+    """The sequences of a call (lfm_kv_batch): own_len [batch], page tables [batch][max_pages],
+    the rows of each sequence's new tokens, and the prefix all of them begin with.  Holds
+    addresses, no memory; the device contents may change between calls."""
+
+    def __init__(self, batch: int, own_len, pages, max_pages: int, max_new: int = 1,
+                 max_len: int | None = None, tokens: int | None = None, new_start=None,
+                 prefix_pages=None, prefix_len: int = 0):
+        self._keep = (own_len, pages, new_start, prefix_pages)
+        self.c = _native.LfmKvBatch(batch, batch * max_new if tokens is None else tokens, max_new,
+                                    0 if max_len is None else max_len, _ptr(new_start),
+                                    _ptr(own_len), _ptr(pages), max_pages, _ptr(prefix_pages),
+                                    prefix_len)
+        self.ref = ctypes.byref(self.c)
+
+
+def kv_write(cache: KVCache, batch: KVBatch, qkv, ld, heads=HEADS, k_col=Q_COLS,
+             v_col=Q_COLS + KV_COLS, q_weight=None, k_weight=None, cos=None, sin=None, max_pos=0,
+             bad_flag=None, stream=None):
+    _ck(_native.lib().lfm_kv_write(cache.ref, batch.ref, _ptr(qkv), ld, heads, k_col, v_col,
+                                   _ptr(q_weight), _ptr(k_weight), _ptr(cos), _ptr(sin), max_pos,
+                                   _ptr(bad_flag), _stream(stream)), "lfm_kv_write")
+
+
+def kv_read(cache: KVCache, batch: KVBatch, k_out, v_out, rows, ld=None, bad_flag=None,
+            stream=None):
+    _ck(_native.lib().lfm_kv_read(cache.ref, batch.ref, _ptr(k_out), _ptr(v_out), rows,
+                                  cache.c.kv_heads * HEAD_DIM if ld is None else ld,
+                                  _ptr(bad_flag), _stream(stream)), "lfm_kv_read")
+
+
+def kv_attention_workspace(cache: KVCache, batch: KVBatch, heads=HEADS) -> int:
+    n = ctypes.c_size_t(0)
+    _ck(_native.lib().lfm_kv_attention_workspace(cache.ref, batch.ref, heads, ctypes.byref(n)),
+        "lfm_kv_attention_workspace")
+    return n.value
+
+
+def kv_attention(cache: KVCache, batch: KVBatch, qkv, ld, out, heads=HEADS, ld_out=None,
+                 workspace=None, workspace_bytes=0, bad_flag=None, stream=None):
+    _ck(_native.lib().lfm_kv_attention(cache.ref, batch.ref, _ptr(qkv), ld, _ptr(out),
+                                       heads * HEAD_DIM if ld_out is None else ld_out, heads,
+                                       _ptr(workspace), workspace_bytes, _ptr(bad_flag),
+                                       _stream(stream)), "lfm_kv_attention")
+
+
+def softmax_workspace(rows, dim) -> int:
+    n = ctypes.c_size_t(0)
+    _ck(_native.lib().lfm_softmax_workspace(rows, dim, ctypes.byref(n)), "lfm_softmax_workspace")
+    return n.value
+
+
+def softmax(x, y, rows, dim, temperature=1.0, x_stride=None, y_stride=None, workspace=None,
+            workspace_bytes=0, stream=None):
+    _ck(_native.lib().lfm_softmax(_ptr(x), dim if x_stride is None else x_stride, _ptr(y),
+                                  dim if y_stride is None else y_stride, rows, dim, temperature,
+                                  _ptr(workspace), workspace_bytes, _stream(stream)), "lfm_softmax")
+
+
+def verify_draft_workspace(batch, vocab) -> int:
+    n = ctypes.c_size_t(0)
+    _ck(_native.lib().lfm_verify_draft_workspace(batch, vocab, ctypes.byref(n)),
+        "lfm_verify_draft_workspace")
+    return n.value
+
+
+def verify_draft(target, draft, draft_ids, u_accept, u_sample, accepted, tokens, batch, n_draft,
+                 vocab, n_valid=None, workspace=None, workspace_bytes=0, stream=None):
+    _ck(_native.lib().lfm_verify_draft(_ptr(target), _ptr(draft), _ptr(draft_ids), _ptr(u_accept),
+                                       _ptr(u_sample), _ptr(n_valid), batch, n_draft, vocab,
+                                       _ptr(accepted), _ptr(tokens), _ptr(workspace),
+                                       workspace_bytes, _stream(stream)), "lfm_verify_draft")
+
+
 def rope_tables(max_pos, head_dim=HEAD_DIM, theta=ROPE_THETA):
     """Host cos/sin tables [max_pos][head_dim] (RotaryEmbedding::init_gpu)."""
     c = np.empty((max_pos, head_dim), np.float32)

@@ -87,6 +87,139 @@ int lfm_attention(const float *qkv, int ld, float *out, int batch, int seq, int 
 int lfm_shortconv(const float *bcg, const float *conv_weight, float *y, int batch, int seq,
                   int hidden, int kernel, moe_stream_t stream);
 
+/* ---- serving: a paged KV cache, and sampling ---------------------------- */
+
+/* How a cache holds keys and values, in rows of 64 (one token, one kv head):
+ *   F32, BF16  the values, bf16 rounded to the nearest (halves to even);
+ *   INT8       s = amax / 127 in fp32, then x / s to the nearest integer
+ *              (halves to even), held to [-127, 127]; a value reads as q * s;
+ *   FP8        s = the least power of two, 2^-126 at least, for which amax / s
+ *              <= 448, then x / s to the nearest e4m3 value; reads as q * s.
+ * amax is the row's largest magnitude; a row of zeros, or so small that INT8's
+ * s is 0, reads as zeros.  An INT8 or FP8 row with an infinity or a NaN reads
+ * as NaN throughout (s = NaN). */
+enum lfm_kv_format { LFM_KV_F32 = 0, LFM_KV_BF16 = 1, LFM_KV_INT8 = 2, LFM_KV_FP8 = 3 };
+
+/* The caller's cache buffers: k and v [num_pages][kv_heads][page_tokens][64] of
+ * the format's type, 16-byte aligned; k_scale and v_scale [num_pages][kv_heads]
+ * [page_tokens] fp32 for INT8 and FP8, NULL for the others.  page_tokens is a
+ * power of two, 16 to 4096.  Nothing has to be initialised. */
+typedef struct lfm_kv_cache {
+  int format;
+  int kv_heads;
+  int page_tokens;
+  int num_pages;
+  void *k, *v;
+  float *k_scale, *v_scale;
+} lfm_kv_cache;
+
+/* The sequences of a call.  Every sequence may begin with the same `prefix_len`
+ * positions, held in prefix_pages [ceil(prefix_len / page_tokens)]; its own
+ * positions follow, own_len[b] of them, in the pages pages[b][0 .. max_pages).
+ * The last n_b own positions are this call's new tokens: rows new_start[b] ..
+ * new_start[b + 1] - 1 of the call's token tensors, or, where new_start is
+ * NULL, rows b * max_new .. b * max_new + max_new - 1.  Pointers are device
+ * memory; own_len, new_start and the tables are read when the kernels run, so a
+ * captured graph follows their contents.
+ *   tokens    rows of the token tensors (new_start NULL: batch * max_new);
+ *   max_new   the most new tokens a sequence has;
+ *   max_len   about the most own positions a sequence has: it decides how the
+ *             work is split, not what is computed.
+ * A sequence whose own_len is 0 takes no part (a slot of a padded batch): its
+ * rows of an output stay as they were.  So does, and sets the call's *bad_flag
+ * (device int, may be NULL) to 1, one whose contents do not fit: own_len below 0
+ * or beyond max_pages * page_tokens; new_start that runs backwards, past
+ * `tokens` or past max_new; more new tokens than own_len.  A page outside
+ * [0, num_pages) sets the flag too: its positions are not written, read as
+ * zeros and take no part in attention.  Pages may be shared for reading; a
+ * position that two tokens of one call are written to holds either's values or
+ * a mixture. */
+typedef struct lfm_kv_batch {
+  int batch;
+  int tokens;
+  int max_new;
+  int max_len;
+  const int *new_start;
+  const int *own_len;
+  const int *pages;
+  int max_pages;
+  const int *prefix_pages;
+  int prefix_len;
+} lfm_kv_batch;
+
+/* Stores the new tokens' keys and values: columns k_col + g*64 and v_col + g*64
+ * of qkv [tokens][ld], g < kv_heads, to the tokens' own positions.  (The shared
+ * prefix is written as the own positions of a batch of one.)  With q_weight,
+ * k_weight, cos_table and sin_table (all or none; `heads` and max_pos are used
+ * only then) q and k are first normalised and rotated as lfm_qk_norm_rope does,
+ * bit for bit, for position prefix_len + own position: q in place in columns
+ * [0, heads*64), k on its way to the cache (qkv keeps its own).  A position of
+ * max_pos, the tables' rows, or more sets *bad_flag and leaves the token out.  qkv 16-byte aligned, ld, k_col and v_col multiples of 4,
+ * heads*64 <= k_col, k_col + kv_heads*64 <= v_col. */
+int lfm_kv_write(const lfm_kv_cache *cache, const lfm_kv_batch *batch, float *qkv, int ld,
+                 int heads, int k_col, int v_col, const float *q_weight, const float *k_weight,
+                 const float *cos_table, const float *sin_table, int max_pos, int *bad_flag,
+                 moe_stream_t stream);
+
+/* Reads own positions back: row b * rows + p of k_out and v_out
+ * [batch * rows][ld] (columns g*64) is position p of sequence b, for p <
+ * min(own_len[b], rows); the other rows stay as they were (new_start,
+ * tokens and max_new play no part).  Either output may be NULL.  ld a multiple
+ * of 4, at least kv_heads * 64. */
+int lfm_kv_read(const lfm_kv_cache *cache, const lfm_kv_batch *batch, float *k_out, float *v_out,
+                int rows, int ld, int *bad_flag, moe_stream_t stream);
+
+/* out[t][h*64 + d] = sum_j softmax_j(q_h(t) . k_g(j) / 8) v_g(j)[d] over the
+ * prefix and the own positions j up to t's own, g = h / (heads / kv_heads): the
+ * attention of lfm_attention for new tokens whose keys and values, their own
+ * included, are in the cache.  q is read from columns [0, heads*64) of qkv
+ * [tokens][ld], out has rows of ld_out.  heads a multiple of kv_heads, at most
+ * 64 of them for each.  A token that sees no position (its pages are outside the
+ * cache) gets zeros.  The prefix's
+ * keys and values are read once for all sequences.  Sums, maxima and weights
+ * are fp32.  A key that is not finite makes the outputs of the tokens that see
+ * it, for its heads, NaN, and a value that is not finite those of its column
+ * not finite; what a token does not see does not reach it.
+ * workspace: lfm_kv_attention_workspace bytes, 16-byte aligned (NULL where that
+ * is 0), the caller's to keep from other calls until this one has run; it needs
+ * no initial contents. */
+int lfm_kv_attention(const lfm_kv_cache *cache, const lfm_kv_batch *batch, const float *qkv,
+                     int ld, float *out, int ld_out, int heads, void *workspace,
+                     size_t workspace_bytes, int *bad_flag, moe_stream_t stream);
+/* Bytes for a call with these arguments (contents of device memory play no part). */
+int lfm_kv_attention_workspace(const lfm_kv_cache *cache, const lfm_kv_batch *batch, int heads,
+                               size_t *bytes);
+
+/* y[r][i] = exp((x[r][i] - max x[r]) / temperature) / sum: probabilities of the
+ * logits of `rows` rows of `dim`, row r at x + r*x_stride and y + r*y_stride
+ * (floats).  A logit of -infinity gives 0, a row of nothing else zeros; NaN or
+ * +infinity makes its row NaN.  temperature > 0.  y may be x (with equal
+ * strides); otherwise the two do not overlap. */
+int lfm_softmax(const float *x, long long x_stride, float *y, long long y_stride, int rows, int dim,
+                float temperature, void *workspace, size_t workspace_bytes, moe_stream_t stream);
+int lfm_softmax_workspace(int rows, int dim, size_t *bytes);
+
+/* Verification of drafted tokens.  target [batch][n_draft + 1][vocab] holds the
+ * target's probabilities after each draft (row 0: before the first), draft
+ * [batch][n_draft][vocab] those that draft_ids [batch][n_draft] were drawn from,
+ * u_accept [batch][n_draft] and u_sample [batch] random numbers of [0, 1);
+ * n_valid [batch] how many drafts a sequence has (NULL: n_draft for all; held
+ * to [0, n_draft]).  Draft i is accepted if all before it were and
+ * u_accept * draft[i][id] < target[i][id].  Then one more token is drawn: after
+ * a rejected draft i from max(target[i] - draft[i], 0), or from target[i] where
+ * that has no positive sum; after n_valid accepted drafts from target[n_valid].
+ * It is the lowest id up to which the weights' sum exceeds u_sample times their
+ * whole sum, in 64 bits; -1 where no weight is positive.  Weights that are NaN
+ * or below 0 count as 0, and an id outside [0, vocab) is rejected.
+ * accepted [batch] = the number of accepted drafts; tokens [batch][n_draft + 1]
+ * = these, the drawn token, then -1.  n_draft = 0 draws one token from target
+ * (draft, draft_ids and u_accept may then be NULL). */
+int lfm_verify_draft(const float *target, const float *draft, const int *draft_ids,
+                     const float *u_accept, const float *u_sample, const int *n_valid, int batch,
+                     int n_draft, int vocab, int *accepted, int *tokens, void *workspace,
+                     size_t workspace_bytes, moe_stream_t stream);
+int lfm_verify_draft_workspace(int batch, int vocab, size_t *bytes);
+
 /* Rotary tables [max_pos][head_dim] in host memory, computed as
  * RotaryEmbedding::init_gpu does (layer.cu:1167-1178): theta_j =
  * powf(theta, -2.0f*j/head_dim), angle = (float)i * theta_j, cos/sin of the

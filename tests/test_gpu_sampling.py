@@ -1,0 +1,213 @@
+"""Softmax of logits and verification of drafted tokens on the GPU against plain numpy
+in 64 bits (kv_ref)."""
+import sys
+
+import numpy as np
+import pytest
+
+import kv_ref as R
+from conftest import bits
+
+EPS = 2.0 ** -24
+
+
+def say(*a):
+    print(*a, flush=True)
+    sys.stdout.flush()
+
+
+def dev(a):
+    from final_amd import hip
+    return hip.DeviceArray.from_numpy(np.ascontiguousarray(a))
+
+
+def run_softmax(dx, dy, rows, dim, t, **kw):
+    from final_amd import hip, lfm
+    need = lfm.softmax_workspace(rows, dim)
+    ws = hip.DeviceArray((max(need, 16),), np.uint8)
+    ws.fill_async(0xFF)
+    lfm.softmax(dx, dy, rows, dim, temperature=t, workspace=ws, workspace_bytes=need, **kw)
+    return dy.download()
+
+
+def close(got, x, t):
+    """A weight's exponent, at most |a| = (max - x) / t, takes three roundings (the difference, 1 / t, the
+    product), so the weight is off by 3 |a| and 3 for exp itself; the sum by as much on average over
+    the weights and log2(dim) + 70 for its additions (threads sum at most 64 each); the quotient by 3.
+    Below 2^-126 by two steps of the subnormal grid, or all of it."""
+    ref = R.softmax(x, t)
+    with np.errstate(invalid="ignore"):
+        a = (x.astype(np.float64).max(1, keepdims=True) - x) / np.float64(np.float32(t))
+    a = np.where(ref > 0, np.minimum(a, 800.0), 0.0)
+    of_sum = (ref * (3 * a + 3)).sum(1, keepdims=True) + np.log2(x.shape[1] + 1) + 70
+    tol = ref * EPS * (3 * a + 6 + of_sum) + 2.0 ** -126
+    assert np.array_equal(np.isfinite(got), np.isfinite(ref))
+    err = np.abs(got - ref)
+    assert (err <= tol).all(), float((err / tol).max())
+    assert np.all(got[ref == 0] <= 2.0 ** -126)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,dim", [(1, 1), (3, 2), (1, 65536), (2, 65537), (5, 1000), (1, 4099), (300, 4096),
+                                      (17, 16385), (257, 8191), (1, 150001), (260, 65539), (64, 65536)])
+@pytest.mark.parametrize("t", [1.0, 0.3])
+def test_softmax(rows, dim, t):
+    say(f"[softmax] rows={rows} dim={dim} t={t}")
+    r = np.random.default_rng(rows + dim)
+    x = 3 * r.standard_normal((rows, dim), dtype=np.float32)
+    x[0, dim // 2] = 40.0
+    close(run_softmax(dev(x), dev(np.zeros_like(x)), rows, dim, t), x, t)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,dim", [(4, 700), (4, 65536), (300, 9001)])
+def test_softmax_of_masks_and_extremes(rows, dim):
+    r = np.random.default_rng(dim)
+    x = r.standard_normal((rows, dim), dtype=np.float32)
+    x[0, ::3] = -np.inf
+    x[1] = -np.inf
+    x[2, 5:] = np.finfo(np.float32).min  # the lowest value as a mask
+    x[3] = np.finfo(np.float32).max
+    x[3, 1] = -np.finfo(np.float32).max
+    got = run_softmax(dev(x), dev(np.zeros_like(x)), rows, dim, 0.7)
+    close(got, x, 0.7)
+    assert not got[1].any() and not got[2, 5:].any() and got[3, 1] == 0
+    x[0, 7], x[2, 0], x[3, 0] = np.nan, np.inf, -np.inf
+    bad = run_softmax(dev(x), dev(np.zeros_like(x)), rows, dim, 0.7)
+    assert np.isnan(bad[[0, 2]]).all() and np.isfinite(bad[3]).all() and not bad[1].any()
+    if rows > 4:  # the other rows keep their bits
+        assert np.array_equal(bits(bad[4:]), bits(got[4:]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,dim,xs,ys,shift", [(3, 1000, 1003, 1001, 1), (2, 65536, 65540, 65536, 0), (260, 513, 513, 520, 3)])
+def test_softmax_strides_and_in_place(rows, dim, xs, ys, shift):
+    from final_amd import hip
+    r = np.random.default_rng(dim)
+    flat = r.standard_normal(rows * xs + 8, dtype=np.float32)
+    dx, out = dev(flat), np.full(rows * ys + 8, 7.0, np.float32)
+    dy = dev(out)
+    x = np.stack([flat[shift + i * xs:shift + i * xs + dim] for i in range(rows)])
+    from final_amd import lfm
+    need = lfm.softmax_workspace(rows, dim)
+    ws = hip.DeviceArray((max(need, 16),), np.uint8)
+    lfm.softmax(dx.ptr + 4 * shift, dy.ptr + 4 * shift, rows, dim, temperature=0.9, x_stride=xs, y_stride=ys, workspace=ws,
+                workspace_bytes=need)
+    got = dy.download()
+    y = np.stack([got[shift + i * ys:shift + i * ys + dim] for i in range(rows)])
+    close(y, x, 0.9)
+    mask = np.ones(len(got), bool)
+    for i in range(rows):
+        mask[shift + i * ys:shift + i * ys + dim] = False
+    assert (got[mask] == 7.0).all() and np.array_equal(bits(dx.download()), bits(flat))
+    lfm.softmax(dx.ptr + 4 * shift, dx.ptr + 4 * shift, rows, dim, temperature=0.9, x_stride=xs, workspace=ws,
+                y_stride=xs, workspace_bytes=need)
+    got = dx.download()
+    assert np.array_equal(bits(np.stack([got[shift + i * xs:shift + i * xs + dim] for i in range(rows)])), bits(y))
+
+
+# -- verification ---------------------------------------------------------------
+
+def probs(r, *shape, sharp=2.0):
+    x = sharp * r.standard_normal(shape)
+    e = np.exp(x - x.max(-1, keepdims=True))
+    return (e / e.sum(-1, keepdims=True)).astype(np.float32)
+
+
+def run_verify(t, d, ids, ua, us, n=None, vocab=None):
+    from final_amd import hip, lfm
+    B, K1, V = t.shape
+    keep = [dev(a) if a is not None and a.size else None for a in (t, d, ids, ua, us, n)]
+    acc, tok = dev(np.full(B, -9, np.int32)), dev(np.full((B, K1), -9, np.int32))
+    need = lfm.verify_draft_workspace(B, V)
+    ws = hip.DeviceArray((max(need, 16),), np.uint8)
+    ws.fill_async(0xFF)
+    lfm.verify_draft(keep[0], keep[1], keep[2], keep[3], keep[4], acc, tok, B, K1 - 1, V, n_valid=keep[5], workspace=ws,
+                     workspace_bytes=need)
+    return acc.download(), tok.download()
+
+
+def same(got, want):
+    assert np.array_equal(got[0], want[0]) and np.array_equal(got[1], want[1]), (got, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,K,V", [(1, 0, 1), (1, 4, 65536), (3, 1, 2), (7, 3, 1001), (64, 4, 4096), (2, 8, 65537),
+                                   (5, 0, 150001), (300, 2, 700), (33, 16, 999)])
+def test_verify(B, K, V):
+    say(f"[verify] B={B} K={K} V={V}")
+    r = np.random.default_rng(B + K + V)
+    t = probs(r, B, K + 1, V)
+    d = (0.8 * t[:, :K] + 0.2 * probs(r, B, K, V)).astype(np.float32)
+    ids = np.array([[R.draw(d[b, i].astype(np.float64), r.random()) for i in range(K)] for b in range(B)],
+                   np.int32).reshape(B, K)
+    ua, us = r.random((B, K), dtype=np.float32), r.random(B, dtype=np.float32)
+    n = np.full(B, K, np.int32)
+    want = R.verify(t, d, ids, ua, us, n)
+    same(run_verify(t, d, ids, ua, us), want)
+    n = r.integers(-2, K + 3, B).astype(np.int32)  # held to [0, K]
+    same(run_verify(t, d, ids, ua, us, n), R.verify(t, d, ids, ua, us, n))
+    if B == 64:
+        assert 0 < want[0].mean() < K  # both outcomes were there
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("V", [5, 1000, 65536, 70001])
+def test_verify_borders(V):
+    """Equal distributions, one-hot ones, zeros, random numbers at both ends, ids outside, NaN and negative weights."""
+    r = np.random.default_rng(V)
+    K = 2
+    top = np.nextafter(np.float32(1), np.float32(0))
+    t, d = probs(r, 12, K + 1, V), probs(r, 12, K, V)
+    ids = r.integers(0, V, (12, K)).astype(np.int32)
+    ua, us = np.full((12, K), 0.5, np.float32), np.array([0, top] * 6, np.float32)
+    d[0] = t[0, :K]                      # equal: u < 1 accepts both
+    d[1], ua[1] = t[1, :K], top
+    t[2, 0], d[2, 0], ids[2, 0] = 0, 0, 1   # 0 < 0: rejected, nothing to draw from
+    t[3, 0], t[3, 0, V - 1], ids[3, 0] = 0, 1, V - 1  # one-hot on the last id
+    d[3, 0], t[3, 1], t[3, 1, V - 2], ids[3, 1] = 0.25 / V, 0, 1, 0
+    ids[4, 0], ids[5, 0], ids[6, 1] = -1, V, 1 << 30
+    t[7, 0, ::2], t[7, 0, 1] = np.nan, -3.0
+    ids[7, 0] = 0
+    t[8, 0], d[8, 0], ids[8, 0] = d[8, 0], t[8, 0], 3
+    t[9, 0], d[9, 0] = t[9, 0] * np.float32(0.5), 1.0  # never above the draft: drawn from the target
+    ids[9, 0], ua[9, 0] = 2, top
+    t[10, 0, 4:], us[10] = 0, top
+    ua[11], d[11, :, :] = 0, 0           # a draft of probability 0 under u = 0
+    with np.errstate(invalid="ignore"):
+        want = R.verify(t, d, ids, ua, us, np.full(12, K))
+    assert want[0][0] == want[0][1] == 2 and want[1][2, 0] == -1 and want[0][3] == 1 and want[1][9, 0] >= 0
+    same(run_verify(t, d, ids, ua, us), want)
+
+
+@pytest.mark.gpu
+def test_verify_of_many_random_numbers():
+    """One distribution at many random numbers: every id is drawn at its place of the running sum."""
+    r = np.random.default_rng(0)
+    V, B = 3001, 2000
+    p = probs(r, V)
+    t = np.broadcast_to(p, (B, 1, V))
+    us = np.sort(r.random(B, dtype=np.float32))
+    got = run_verify(np.ascontiguousarray(t), None, None, None, us)
+    want = R.verify(np.ascontiguousarray(t), None, None, None, us, np.zeros(B))
+    same(got, want)
+
+
+@pytest.mark.gpu
+def test_logits_to_verified_tokens():
+    """Head logits of drafts through softmax (in place) and verification, as a step with drafts runs them."""
+    from final_amd import lfm
+    r = np.random.default_rng(4)
+    B, K, V = 6, 3, lfm.VOCAB
+    logits = (2 * r.standard_normal((B * (K + 1), V))).astype(np.float32)
+    dl = (logits.reshape(B, K + 1, V)[:, :K] + 0.5 * r.standard_normal((B, K, V))).astype(np.float32).reshape(B * K, V)
+    t, d = dev(logits), dev(dl)
+    pt = run_softmax(t, t, B * (K + 1), V, 0.8).reshape(B, K + 1, V)
+    pd = run_softmax(d, d, B * K, V, 0.8).reshape(B, K, V)
+    us = r.random(B, dtype=np.float32)
+    # the drafts: one token each from the draft's probabilities, by the same operator
+    ids = np.stack([run_verify(np.ascontiguousarray(pd[:, i:i + 1]), None, None, None, r.random(B, dtype=np.float32))[1][:, 0]
+                    for i in range(K)], 1).astype(np.int32)
+    assert (ids >= 0).all()
+    ua = r.random((B, K), dtype=np.float32)
+    same(run_verify(pt, pd, ids, ua, us), R.verify(pt, pd, ids, ua, us, np.full(B, K)))
