@@ -31,7 +31,8 @@ int kv_args(const lfm_kv_cache *c, const lfm_kv_batch *b, int *bad, lfm::KvArgs 
   if (c->kv_heads > 256) return MOE_ERR_UNSUPPORTED;
   if (!c->k || !c->v || !al16(c->k) || !al16(c->v)) return MOE_ERR_INVALID_ARG;
   const bool scaled = c->format == LFM_KV_INT8 || c->format == LFM_KV_FP8;
-  if (scaled != (c->k_scale != nullptr) || scaled != (c->v_scale != nullptr))
+  if (scaled != (c->k_scale != nullptr) || scaled != (c->v_scale != nullptr) || !al16(c->k_scale) ||
+      !al16(c->v_scale))
     return MOE_ERR_INVALID_ARG;
   if (b->batch < 0 || b->tokens < 0 || b->max_new < 0 || b->max_len < 0 || b->max_pages < 0 ||
       b->prefix_len < 0)
@@ -53,7 +54,8 @@ int kv_args(const lfm_kv_cache *c, const lfm_kv_batch *b, int *bad, lfm::KvArgs 
 
 int kv_heads_ok(const lfm::KvArgs &a, int heads) {
   if (heads <= 0 || heads % a.kv_heads != 0) return MOE_ERR_INVALID_ARG;
-  if (heads / a.kv_heads > 64 || (long long)a.max_new * heads >> 24) return MOE_ERR_UNSUPPORTED;
+  if (heads / a.kv_heads > 64 || (long long)a.max_new * heads >> 24 || (long long)a.tokens * heads >> 30)
+    return MOE_ERR_UNSUPPORTED;
   return MOE_OK;
 }
 

@@ -6,6 +6,7 @@
 
 #include "lfm_kv.h"
 #include "lfm_rope.h"
+#include "split_tile.h"
 
 namespace lfm {
 
@@ -102,59 +103,498 @@ __global__ __launch_bounds__(256) void kv_read_kernel(KvArgs a, float *k_out, fl
 // ---------------------------------------------------------------------------
 // Attention over the cache
 // ---------------------------------------------------------------------------
+//
+// A wave computes S^T = K Q^T and O^T = V^T P^T on v_mfma_f32_16x16x32_bf16 for
+// tiles of 32 keys and CT tiles of 16 columns, a column being one query head of
+// one token that attends the kv head's keys: the heads of a group and the new
+// tokens of a sequence (or, for the prefix, of all sequences) stand next to each
+// other.  q is the exact sum of three bf16 parts, as is a weight p, and int8,
+// e4m3 and bf16 keys and values are bf16 values as they are (an fp32 cache's are
+// split too, six of the nine products taken), so the products are exact, their
+// sums fp32, and the rows' scales are applied to scores and weights in fp32.
+//
+// Nothing is staged in LDS and nothing transposed: a lane (c = l % 16, g = l / 16)
+// loads 16 bytes of key c of each half tile, which is its operand of S^T up to a
+// permutation of the dimensions (the same in q's), and four values, dimensions 4c
+// .. 4c+3, of the keys 4g + i, whose weights S^T leaves in this lane: block db of
+// O^T takes dimension 4c + db from each.  The four waves of a block take every
+// fourth tile and join their sums through LDS at the end.
+//
+// The running maximum is only raised when a score passes it by kRaise: weights
+// then reach 2^kRaise, and most tiles need no exchange between lanes and no
+// scaling of O.
 
-// One wave per (new token, query head): 64 positions at a time, a lane's
-// position for the scores, a lane's column for the values.
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kKeys = 32;           // keys per tile
+constexpr int kFlashWaves = 4;
+constexpr int kFlashThreads = 64 * kFlashWaves;
+constexpr int kMinTiles = 8;        // tiles of a split, at least
+constexpr float kRaise = 8.0f;      // log2
+constexpr int kJoinPitch = 68;      // floats per column of the joined O
+constexpr float kNoScore = -__builtin_inff();
+
+struct FlashArgs {
+  const float *q;
+  float *out;
+  float *po;   // [parts][rows][64]: sums of p v of a part
+  float2 *pm;  // [parts][rows]: its maximum (log2) and sum of p
+  int ld, ldo, heads, group;
+  int own_parts, prefix_parts;  // parts 0 .. own_parts are the own positions'
+  size_t rows;                  // tokens * heads
+};
+
+// Tiles per part when `n` keys are split into at most `parts`.
+__host__ __device__ inline int part_tiles(int n, int parts) {
+  const int tiles = (n + kKeys - 1) / kKeys, per = (tiles + parts - 1) / parts;
+  return (max(per, kMinTiles) + kFlashWaves - 1) / kFlashWaves * kFlashWaves;
+}
+
+// Keys and values of a tile as they were loaded.
 template <int FMT>
-__global__ __launch_bounds__(64) void kv_attention_kernel(KvArgs a, const float *q, int ld, float *out,
-                                                          int ldo, int heads) {
+struct RawTile {
+  static constexpr int KW = FMT == LFM_KV_F32 ? 4 : FMT == LFM_KV_BF16 ? 2 : 1;  // 16-byte loads of a key's quarter
+  static constexpr bool SCALED = FMT == LFM_KV_INT8 || FMT == LFM_KV_FP8;
+  u32x4 k[2][KW];
+  uint32_t v[2][4][KW];  // [half][key 4g + i][dwords]
+  f32x4 ks[2], vs[2];    // scales of keys 4g .. 4g+3
+  bool ok[2];            // the half's page is inside the cache
+};
+
+// Dimension of element j of k-step s in a lane of group g (K's loads decide it).
+template <int FMT>
+__device__ __forceinline__ constexpr int key_dim(int s, int g, int j) {
+  return FMT == LFM_KV_F32    ? 32 * s + 16 * (j >> 2) + 4 * g + (j & 3)
+         : FMT == LFM_KV_BF16 ? 32 * s + 8 * g + j
+                              : 16 * g + 8 * s + j;
+}
+
+__device__ __forceinline__ uint32_t pack_hi(uint32_t lo, uint32_t hi) {  // upper halves of two floats
+  return __builtin_amdgcn_perm(hi, lo, 0x07060302u);
+}
+
+__device__ __forceinline__ uint32_t byte_pair(float lo, float hi) {  // two small integers as bf16, exactly
+  return pack_hi(__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi));
+}
+
+// Bits 0 and 1 as masks of a dword's halves.
+__device__ __forceinline__ uint32_t half_mask(uint32_t bits) {
+  return (bits & 1u ? 0xFFFFu : 0u) | (bits & 2u ? 0xFFFF0000u : 0u);
+}
+
+// Four bytes of an 8-bit format -> two dwords of bf16.
+template <int FMT>
+__device__ __forceinline__ void widen4(uint32_t w, uint32_t &lo, uint32_t &hi) {
+  if constexpr (FMT == LFM_KV_FP8) {
+    lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, false));
+    hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, true));
+  } else {
+    lo = byte_pair((float)(signed char)w, (float)(signed char)(w >> 8));
+    hi = byte_pair((float)(signed char)(w >> 16), (float)(signed char)(w >> 24));
+  }
+}
+
+// Three parts of eight floats, each exact in bf16 together (truncation: 8 bits a part).
+__device__ __forceinline__ void split8_exact(const float (&x)[8], bf16x8 (&part)[3]) {
+  u32x4 p[3];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    uint32_t a0 = __builtin_bit_cast(uint32_t, x[2 * j]), b0 = __builtin_bit_cast(uint32_t, x[2 * j + 1]);
+    const float a1 = x[2 * j] - __builtin_bit_cast(float, a0 & 0xFFFF0000u);
+    const float b1 = x[2 * j + 1] - __builtin_bit_cast(float, b0 & 0xFFFF0000u);
+    const uint32_t ua = __builtin_bit_cast(uint32_t, a1), ub = __builtin_bit_cast(uint32_t, b1);
+    const float a2 = a1 - __builtin_bit_cast(float, ua & 0xFFFF0000u);
+    const float b2 = b1 - __builtin_bit_cast(float, ub & 0xFFFF0000u);
+    p[0][j] = pack_hi(a0, b0);
+    p[1][j] = pack_hi(ua, ub);
+    p[2][j] = byte_pair(a2, b2);
+  }
+#pragma unroll
+  for (int q = 0; q < 3; ++q) part[q] = __builtin_bit_cast(bf16x8, p[q]);
+}
+
+// acc += the product of an operand of NP parts with one of three.
+template <int NP>
+__device__ __forceinline__ f32x4 mfma_parts(const bf16x8 (&x)[NP], const bf16x8 (&y)[3], f32x4 acc) {
+  if constexpr (NP == 1) {
+#pragma unroll
+    for (int q = 2; q >= 0; --q) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[0], y[q], acc, 0, 0, 0);
+  } else {
+#pragma unroll
+    for (int m = 0; m < moe::kSplitProducts; ++m)
+      acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[moe::kSplitA[m]], y[moe::kSplitB[m]], acc, 0, 0, 0);
+  }
+  return acc;
+}
+
+template <int FMT, int CT, bool PREFIX>
+__global__ __launch_bounds__(kFlashThreads) __attribute__((amdgpu_waves_per_eu(CT == 1 ? 3 : 2)))
+void kv_flash_kernel(KvArgs a, FlashArgs f) {
+  using Raw = RawTile<FMT>;
+  constexpr int NP = FMT == LFM_KV_F32 ? 3 : 1;
+  __shared__ float s_o[kFlashWaves][CT * 16 * kJoinPitch];
+  __shared__ float2 s_m[kFlashWaves][CT * 16];
+  const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // kv head fastest: with 8 of them a head's keys stay in one XCD's L2
+  const int h = blockIdx.x % a.kv_heads, part = blockIdx.x / a.kv_heads;
+  const int col0 = blockIdx.y * CT * 16;
+
   KvSeq s;
-  if (!kv_seq<true>(a, blockIdx.y, s)) return;
-  const int i = blockIdx.x / heads, h = blockIdx.x - i * heads;
-  if (i >= s.n) return;
-  const int lane = threadIdx.x, g = h / (heads / a.kv_heads);
-  const int end = a.prefix_len + s.len - s.n + i + 1;
-  const float *qr = q + (size_t)(s.row0 + i) * ld + h * kRowDim;
-  float m = -__builtin_inff(), l = 0.0f, o = 0.0f;
-  for (int j0 = 0; j0 < end; j0 += 64) {
-    const int j = j0 + lane, p = j < a.prefix_len ? j : j - a.prefix_len;
-    int page = -1;
-    if (j < end) {
-      page = j < a.prefix_len ? a.prefix_pages[p >> a.pshift]
-                              : a.pages[(size_t)blockIdx.y * a.max_pages + (p >> a.pshift)];
-      if (page < 0 || page >= a.num_pages) {
-        kv_flag(a.bad);
-        page = -1;
+  const int *table;
+  int len, first_seen;  // keys; those below first_seen are seen by every column of the block
+  if (PREFIX) {
+    s.row0 = 0;
+    s.n = a.tokens;
+    table = a.prefix_pages;
+    len = first_seen = a.prefix_len;
+  } else {
+    if (!kv_seq<true>(a, blockIdx.z, s)) return;
+    table = a.pages + (size_t)blockIdx.z * a.max_pages;
+    len = s.len;
+    first_seen = len - s.n + col0 / f.group + 1;
+  }
+  if (col0 >= s.n * f.group) return;
+  const int per = part_tiles(len, PREFIX ? f.prefix_parts : f.own_parts);
+  if (part * per * kKeys >= len) return;
+  const bool direct = !PREFIX && f.prefix_parts == 0 && per * kKeys >= len;
+  // the last position a column of the block sees
+  const int seen = PREFIX ? len : min(len, len - s.n + (col0 + CT * 16 - 1) / f.group + 1);
+  const int t_end = min((part + 1) * per, (seen + kKeys - 1) / kKeys);
+
+  // q's parts, scaled so that a score is the log2 of its weight
+  bf16x8 qp[CT][2][3];
+  int last[CT];  // last position the lane's columns see
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    const int col = col0 + ct * 16 + c, tok = col / f.group, qh = h * f.group + col - tok * f.group;
+    const bool valid = tok < s.n;
+    last[ct] = PREFIX ? len - 1 : len - s.n + tok;
+    const float *qr = f.q + (size_t)(s.row0 + (valid ? tok : 0)) * f.ld + qh * kRowDim;
+#pragma unroll
+    for (int st = 0; st < 2; ++st) {
+      float x[8];
+#pragma unroll
+      for (int j = 0; j < 8; j += 4) {
+        const f32x4 v = moe::ld4(qr + key_dim<FMT>(st, g, j));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[j + e] = valid ? v[e] * (0.125f * 1.44269504088896340736f) : 0.0f;
       }
-    }
-    const size_t row = page >= 0 ? kv_row(a, page, g, p & ((1 << a.pshift) - 1)) : 0;
-    float sc = -__builtin_inff();
-    if (page >= 0) {
-      sc = 0.0f;
-      for (int c = 0; c < 16; ++c) {
-        const f32x4 kv = kv_load_row<FMT>(a.k, a.ks, row, c), qv = moe::ld4(qr + 4 * c);
-        for (int e = 0; e < 4; ++e) sc = __builtin_fmaf(kv[e], qv[e], sc);
-      }
-      sc *= 0.125f;
-    }
-    float mt = sc;
-    for (int d = 32; d > 0; d >>= 1) mt = fmaxf(mt, __shfl_xor(mt, d));
-    const float mn = fmaxf(m, mt), ref = mn == -__builtin_inff() ? 0.0f : mn;
-    const float al = expf(m - ref), e = page >= 0 ? expf(sc - ref) : 0.0f;
-    l = l * al + e;
-    o *= al;
-    m = mn;
-    for (int t = 0; t < 64; ++t) {
-      const int pg = __shfl(page, t);
-      if (pg < 0) continue;
-      const int pt = __shfl(p, t);
-      const float w = __shfl(e, t);
-      const size_t r = kv_row(a, pg, g, pt & ((1 << a.pshift) - 1));
-      o = __builtin_fmaf(w, kv_load_row<FMT>(a.v, a.vs, r, lane >> 2)[lane & 3], o);
+      split8_exact(x, qp[ct][st]);
     }
   }
-  for (int d = 32; d > 0; d >>= 1) l += __shfl_xor(l, d);
-  out[(size_t)(s.row0 + i) * ldo + h * kRowDim + lane] = l == 0.0f ? 0.0f : o / l;
+
+  f32x4 o[CT][4];
+  float m[CT], l[CT];
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    m[ct] = kNoScore;
+    l[ct] = 0.0f;
+#pragma unroll
+    for (int d = 0; d < 4; ++d) o[ct][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+
+  auto load = [&](int t, Raw &r) {
+#pragma unroll
+    for (int hb = 0; hb < 2; ++hb) {
+      const int k0 = min(t * kKeys + 16 * hb, (len - 1) & ~15);
+      int page = __builtin_amdgcn_readfirstlane(table[k0 >> a.pshift]);
+      r.ok[hb] = page >= 0 && page < a.num_pages;
+      if (!r.ok[hb]) {
+        kv_flag(a.bad);
+        page = 0;
+      }
+      const size_t row = kv_row(a, page, h, k0 & ((1 << a.pshift) - 1));
+      const char *kp = a.k + row * kRowDim * kv_size<FMT>(), *vp = a.v + row * kRowDim * kv_size<FMT>();
+#pragma unroll
+      for (int w = 0; w < Raw::KW; ++w)
+        r.k[hb][w] = *reinterpret_cast<const u32x4 *>(kp + c * kRowDim * kv_size<FMT>() + 64 * w + 16 * g);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t *p = reinterpret_cast<const uint32_t *>(vp + ((4 * g + i) * kRowDim + 4 * c) * kv_size<FMT>());
+#pragma unroll
+        for (int w = 0; w < Raw::KW; ++w) r.v[hb][i][w] = p[w];
+      }
+      if constexpr (Raw::SCALED) {
+        r.ks[hb] = moe::ld4(a.ks + row + 4 * g);
+        r.vs[hb] = moe::ld4(a.vs + row + 4 * g);
+      }
+    }
+  };
+
+  auto compute = [&](int t, Raw &r) {
+    const int k0 = t * kKeys;
+    const bool cut = k0 + kKeys > first_seen || !r.ok[0] || !r.ok[1];  // wave-uniform
+    // operands of K
+    bf16x8 kop[2][2][NP];
+#pragma unroll
+    for (int hb = 0; hb < 2; ++hb)
+#pragma unroll
+      for (int st = 0; st < 2; ++st) {
+        if constexpr (FMT == LFM_KV_F32) {
+          const f32x4 x[2] = {__builtin_bit_cast(f32x4, r.k[hb][2 * st]), __builtin_bit_cast(f32x4, r.k[hb][2 * st + 1])};
+          moe::split8(x, kop[hb][st]);
+        } else if constexpr (FMT == LFM_KV_BF16) {
+          kop[hb][st][0] = __builtin_bit_cast(bf16x8, r.k[hb][st]);
+        } else {
+          u32x4 w;
+          uint32_t lo, hi;
+          widen4<FMT>(r.k[hb][0][2 * st], lo, hi);
+          w[0] = lo;
+          w[1] = hi;
+          widen4<FMT>(r.k[hb][0][2 * st + 1], lo, hi);
+          w[2] = lo;
+          w[3] = hi;
+          kop[hb][st][0] = __builtin_bit_cast(bf16x8, w);
+        }
+      }
+    // values of keys behind the sequence's end or on no page: zero
+    if (cut) {
+#pragma unroll
+      for (int hb = 0; hb < 2; ++hb)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const bool there = r.ok[hb] && k0 + 16 * hb + 4 * g + i < len;
+#pragma unroll
+          for (int w = 0; w < Raw::KW; ++w) r.v[hb][i][w] = there ? r.v[hb][i][w] : 0u;
+        }
+    }
+    // operands of V: block db takes dimension 4c + db of the lane's eight keys
+    bf16x8 vop[4][NP];
+    if constexpr (FMT == LFM_KV_F32) {
+#pragma unroll
+      for (int db = 0; db < 4; ++db) {
+        f32x4 x[2];
+#pragma unroll
+        for (int hb = 0; hb < 2; ++hb)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[hb][i] = __builtin_bit_cast(float, r.v[hb][i][db]);
+        moe::split8(x, vop[db]);
+      }
+    } else {
+      u32x4 w[4];
+#pragma unroll
+      for (int hb = 0; hb < 2; ++hb) {
+        const uint32_t(&v)[4][Raw::KW] = r.v[hb];
+        if constexpr (FMT == LFM_KV_BF16) {
+#pragma unroll
+          for (int p = 0; p < 2; ++p)
+#pragma unroll
+            for (int db = 0; db < 4; ++db)
+              w[db][2 * hb + p] = __builtin_amdgcn_perm(v[2 * p + 1][db >> 1], v[2 * p][db >> 1],
+                                                        db & 1 ? 0x07060302u : 0x05040100u);
+        } else if constexpr (FMT == LFM_KV_FP8) {
+          uint32_t q[2][2];  // keys 2p and 2p+1, dimensions (0, 1) and (2, 3), byte by byte
+#pragma unroll
+          for (int p = 0; p < 2; ++p) {
+            q[p][0] = __builtin_amdgcn_perm(v[2 * p + 1][0], v[2 * p][0], 0x05010400u);
+            q[p][1] = __builtin_amdgcn_perm(v[2 * p + 1][0], v[2 * p][0], 0x07030602u);
+          }
+#pragma unroll
+          for (int p = 0; p < 2; ++p)
+#pragma unroll
+            for (int db = 0; db < 4; ++db)
+              w[db][2 * hb + p] = __builtin_bit_cast(
+                  uint32_t, db & 1 ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(q[p][db >> 1], 1.0f, true)
+                                   : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(q[p][db >> 1], 1.0f, false));
+        } else {
+#pragma unroll
+          for (int p = 0; p < 2; ++p)
+#pragma unroll
+            for (int db = 0; db < 4; ++db)
+              w[db][2 * hb + p] = byte_pair((float)(signed char)(v[2 * p][0] >> (8 * db)),
+                                            (float)(signed char)(v[2 * p + 1][0] >> (8 * db)));
+        }
+      }
+#pragma unroll
+      for (int db = 0; db < 4; ++db) vop[db][0] = __builtin_bit_cast(bf16x8, w[db]);
+    }
+    // A value that is not finite must not meet the zero weight of a column that
+    // does not see it: such values (a bit each in nf) leave the product and make
+    // the outputs of the columns that do see them NaN.
+    uint32_t nf = 0;
+    bool apart = false;
+    if (FMT != LFM_KV_INT8 && !PREFIX && cut) {
+#pragma unroll
+      for (int db = 0; db < 4; ++db) {
+        const u32x4 w = __builtin_bit_cast(u32x4, vop[db][0]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          nf |= ((w[j] & 0x7F80u) == 0x7F80u ? 1u : 0u) << (8 * db + 2 * j) |
+                ((w[j] & 0x7F800000u) == 0x7F800000u ? 2u : 0u) << (8 * db + 2 * j);
+      }
+      apart = __any(nf != 0);
+      if (apart) {
+#pragma unroll
+        for (int db = 0; db < 4; ++db)
+#pragma unroll
+          for (int q = 0; q < NP; ++q) {
+            u32x4 w = __builtin_bit_cast(u32x4, vop[db][q]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[j] &= ~half_mask(nf >> (8 * db + 2 * j));
+            vop[db][q] = __builtin_bit_cast(bf16x8, w);
+          }
+      }
+    }
+
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+      float p[8];  // scores, then weights, of keys 16 hb + 4g + i
+#pragma unroll
+      for (int hb = 0; hb < 2; ++hb) {
+        f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int st = 0; st < 2; ++st) acc = mfma_parts<NP>(kop[hb][st], qp[ct][st], acc);
+        if constexpr (Raw::SCALED) acc *= r.ks[hb];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) p[4 * hb + i] = acc[i];
+      }
+      if (cut) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (!r.ok[e >> 2] || k0 + 16 * (e >> 2) + 4 * g + (e & 3) > last[ct]) p[e] = kNoScore;
+      }
+      float mt = p[0];
+#pragma unroll
+      for (int e = 1; e < 8; ++e) mt = fmaxf(mt, p[e]);
+      if (__any(mt > m[ct] + kRaise)) {
+        mt = fmaxf(mt, __shfl_xor(mt, 16));
+        mt = fmaxf(mt, __shfl_xor(mt, 32));
+        const float mn = fmaxf(m[ct], mt);
+        const float scale = mn == kNoScore ? 1.0f : __builtin_amdgcn_exp2f(m[ct] - mn);
+        m[ct] = mn;
+        l[ct] *= scale;
+#pragma unroll
+        for (int d = 0; d < 4; ++d) o[ct][d] *= scale;
+      }
+      const float ref = m[ct] == kNoScore ? 0.0f : m[ct];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        p[e] = __builtin_amdgcn_exp2f(p[e] - ref);
+        l[ct] += p[e];
+      }
+      if constexpr (Raw::SCALED) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) p[e] *= r.vs[e >> 2][e & 3];
+        if (cut) {  // a scale there may be anything
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (!r.ok[e >> 2] || k0 + 16 * (e >> 2) + 4 * g + (e & 3) > last[ct]) p[e] = 0.0f;
+        }
+      }
+      bf16x8 pp[3];
+      split8_exact(p, pp);
+#pragma unroll
+      for (int d = 0; d < 4; ++d) o[ct][d] = mfma_parts<NP>(vop[d], pp, o[ct][d]);
+      if (apart) {
+        // how many of them a column sees: a product of ones
+        u32x4 see;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int k = k0 + 16 * (j >> 1) + 4 * g + 2 * (j & 1);
+          see[j] = (k <= last[ct] ? 0x3F80u : 0u) | (k + 1 <= last[ct] ? 0x3F800000u : 0u);
+        }
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+          u32x4 w;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) w[j] = half_mask(nf >> (8 * d + 2 * j)) & 0x3F803F80u;
+          const f32x4 n = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, w),
+                                                                  __builtin_bit_cast(bf16x8, see),
+                                                                  f32x4{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[ct][d][i] = n[i] > 0.0f ? __builtin_nanf("") : o[ct][d][i];
+        }
+      }
+    }
+  };
+
+  // Two tiles in registers: one computed, one on its way.  A load past the
+  // wave's last tile repeats that one (its lines are in L2).
+  const int t0 = part * per + wave;
+  if (t0 < t_end) {
+    Raw ra, rb;
+    const int t_last = t0 + (t_end - 1 - t0) / kFlashWaves * kFlashWaves;
+    load(t0, ra);
+    for (int t = t0; t < t_end; t += 2 * kFlashWaves) {
+      load(min(t + kFlashWaves, t_last), rb);
+      compute(t, ra);
+      if (t + kFlashWaves >= t_end) break;
+      load(min(t + 2 * kFlashWaves, t_last), ra);
+      compute(t + kFlashWaves, rb);
+    }
+  }
+
+  // Join the waves: a common maximum, then sums.  O^T row 4g + i of block db is
+  // dimension 16g + 4i + db.
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    l[ct] += __shfl_xor(l[ct], 16);
+    l[ct] += __shfl_xor(l[ct], 32);
+    if (g == 0) s_m[wave][ct * 16 + c] = float2{m[ct], l[ct]};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      moe::st4(&s_o[wave][(ct * 16 + c) * kJoinPitch + 16 * g + 4 * i],
+               f32x4{o[ct][0][i], o[ct][1][i], o[ct][2][i], o[ct][3][i]});
+  }
+  __syncthreads();
+#pragma unroll
+  for (int n = 0; n < CT; ++n) {
+    const int e = n * kFlashThreads + threadIdx.x, cc = e >> 4, d = (e & 15) * 4;
+    const int col = col0 + cc, tok = col / f.group, qh = h * f.group + col - tok * f.group;
+    if (tok >= s.n) continue;
+    float mw[kFlashWaves], mx = kNoScore, lt = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kFlashWaves; ++w) {
+      mw[w] = s_m[w][cc].x;
+      mx = fmaxf(mx, mw[w]);
+    }
+    f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int w = 0; w < kFlashWaves; ++w) {
+      const float sc = mw[w] == kNoScore ? (s_m[w][cc].y == 0.0f ? 0.0f : 1.0f) : __builtin_amdgcn_exp2f(mw[w] - mx);
+      lt += s_m[w][cc].y * sc;
+      v += moe::ld4(&s_o[w][cc * kJoinPitch + d]) * sc;
+    }
+    const size_t row = (size_t)(s.row0 + tok) * f.heads + qh;
+    if (direct) {
+      moe::st4(f.out + (size_t)(s.row0 + tok) * f.ldo + qh * kRowDim + d, lt == 0.0f ? v * 0.0f : v * (1.0f / lt));
+    } else {
+      const size_t at = (size_t)(PREFIX ? f.own_parts + part : part) * f.rows + row;
+      moe::st4(f.po + at * kRowDim + d, v);
+      if (d == 0) f.pm[at] = float2{mx, lt};
+    }
+  }
+}
+
+// Joins the parts of a token's head: one wave per row, a lane a dimension.
+__global__ __launch_bounds__(256) void kv_join_kernel(KvArgs a, FlashArgs f) {
+  KvSeq s;
+  if (!kv_seq<true>(a, blockIdx.y, s)) return;
+  const int r = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (r >= s.n * f.heads) return;
+  const int own_per = part_tiles(s.len, f.own_parts) * kKeys, own = (s.len + own_per - 1) / own_per;
+  int pre = 0;
+  if (f.prefix_parts > 0) {
+    const int per = part_tiles(a.prefix_len, f.prefix_parts) * kKeys;
+    pre = (a.prefix_len + per - 1) / per;
+  } else if (own == 1) {
+    return;  // written by its one block
+  }
+  const size_t row = (size_t)s.row0 * f.heads + r;
+  const int tok = r / f.heads, qh = r - tok * f.heads;
+  auto at = [&](int p) { return (size_t)(p < own ? p : f.own_parts + p - own) * f.rows + row; };
+  float mx = kNoScore;
+  for (int p = 0; p < own + pre; ++p) mx = fmaxf(mx, f.pm[at(p)].x);
+  float lt = 0.0f, v = 0.0f;
+  for (int p = 0; p < own + pre; ++p) {
+    const float2 ml = f.pm[at(p)];
+    const float sc = ml.x == kNoScore ? (ml.y == 0.0f ? 0.0f : 1.0f) : __builtin_amdgcn_exp2f(ml.x - mx);
+    lt += ml.y * sc;
+    v += f.po[at(p) * kRowDim + lane] * sc;
+  }
+  f.out[(size_t)(s.row0 + tok) * f.ldo + qh * kRowDim + lane] = lt == 0.0f ? 0.0f : v * (1.0f / lt);
 }
 
 // ---------------------------------------------------------------------------
@@ -199,14 +639,77 @@ hipError_t launch_kv_read(const KvArgs &a, float *k_out, float *v_out, int rows,
   return by_format(a.format, [&](auto f) { return kv_read_launch<f()>(a, k_out, v_out, rows, ld, st); });
 }
 
-size_t kv_attention_ws(const KvArgs &, int) { return 0; }
+// How a call is split: column tiles a wave holds, and parts of the own positions
+// and of the prefix so that about kFlashBlocks blocks run.
+constexpr int kFlashBlocks = 1024;
 
-hipError_t launch_kv_attention(const KvArgs &a, const float *q, int ld, float *out, int ldo, int heads, void *,
+struct FlashPlan {
+  int own_ct, prefix_ct, own_groups, prefix_groups, own_parts, prefix_parts;
+};
+
+static int column_tiles(long long cols) { return cols <= 16 ? 1 : cols <= 32 ? 2 : 4; }
+
+static int parts_of(long long keys, long long blocks) {
+  const long long tiles = (keys + kKeys - 1) / kKeys, most = std::max<long long>(1, tiles / kMinTiles);
+  return (int)std::min<long long>({most, std::max<long long>(1, (kFlashBlocks + blocks - 1) / blocks), 256});
+}
+
+static FlashPlan flash_plan(const KvArgs &a, int heads) {
+  FlashPlan p{};
+  const long long group = heads / a.kv_heads, cap = (long long)a.max_pages << a.pshift;
+  const int widest = a.format == LFM_KV_F32 ? 2 : 4;
+  p.own_ct = std::min(widest, column_tiles(a.max_new * group));
+  p.own_groups = (int)((a.max_new * group + 16 * p.own_ct - 1) / (16 * p.own_ct));
+  p.own_parts = parts_of(std::min<long long>(a.max_len ? a.max_len : cap, cap),
+                         (long long)p.own_groups * a.kv_heads * std::max(a.batch, 1));
+  if (a.prefix_len > 0) {
+    p.prefix_ct = std::min(widest, column_tiles(a.tokens * group));
+    p.prefix_groups = (int)((a.tokens * group + 16 * p.prefix_ct - 1) / (16 * p.prefix_ct));
+    p.prefix_parts = parts_of(a.prefix_len, (long long)p.prefix_groups * a.kv_heads);
+  }
+  return p;
+}
+
+static size_t flash_rows(const KvArgs &a, int heads) { return (size_t)a.tokens * heads; }
+
+size_t kv_attention_ws(const KvArgs &a, int heads) {
+  const FlashPlan p = flash_plan(a, heads);
+  const int parts = p.own_parts + p.prefix_parts;
+  return parts == 1 ? 0 : flash_rows(a, heads) * parts * (kRowDim + 2) * sizeof(float);
+}
+
+template <int FMT, bool PREFIX>
+static hipError_t kv_flash_launch(const KvArgs &a, const FlashArgs &f, int ct, dim3 grid, hipStream_t st) {
+  switch (ct) {
+    case 1: hipLaunchKernelGGL((kv_flash_kernel<FMT, 1, PREFIX>), grid, dim3(kFlashThreads), 0, st, a, f); break;
+    case 2: hipLaunchKernelGGL((kv_flash_kernel<FMT, 2, PREFIX>), grid, dim3(kFlashThreads), 0, st, a, f); break;
+    default:
+      if constexpr (FMT != LFM_KV_F32)
+        hipLaunchKernelGGL((kv_flash_kernel<FMT, 4, PREFIX>), grid, dim3(kFlashThreads), 0, st, a, f);
+  }
+  return hipGetLastError();
+}
+
+hipError_t launch_kv_attention(const KvArgs &a, const float *q, int ld, float *out, int ldo, int heads, void *ws,
                                hipStream_t st) {
-  return by_format(a.format, [&](auto f) {
-    hipLaunchKernelGGL((kv_attention_kernel<f()>), dim3(a.max_new * heads, a.batch), dim3(64), 0, st, a, q, ld, out,
-                       ldo, heads);
-    return hipGetLastError();
+  const FlashPlan p = flash_plan(a, heads);
+  const size_t rows = flash_rows(a, heads);
+  float *po = static_cast<float *>(ws);
+  const FlashArgs f{q, out, po, reinterpret_cast<float2 *>(po + rows * (p.own_parts + p.prefix_parts) * kRowDim),
+                    ld, ldo, heads, heads / a.kv_heads, p.own_parts, p.prefix_parts, rows};
+  if (p.own_groups > 65535 || p.prefix_groups > 65535) return hipErrorInvalidValue;
+  return by_format(a.format, [&](auto fmt) -> hipError_t {
+    hipError_t e = hipSuccess;
+    if (p.prefix_parts)
+      e = kv_flash_launch<fmt(), true>(a, f, p.prefix_ct, dim3(a.kv_heads * p.prefix_parts, p.prefix_groups), st);
+    if (e == hipSuccess)
+      e = kv_flash_launch<fmt(), false>(a, f, p.own_ct, dim3(a.kv_heads * p.own_parts, p.own_groups, a.batch), st);
+    if (e == hipSuccess && p.own_parts + p.prefix_parts > 1) {
+      hipLaunchKernelGGL(kv_join_kernel, dim3((unsigned)((a.max_new * (long long)heads + 3) / 4), a.batch), dim3(256), 0,
+                         st, a, f);
+      e = hipGetLastError();
+    }
+    return e;
   });
 }
 

@@ -101,8 +101,8 @@ int lfm_shortconv(const float *bcg, const float *conv_weight, float *y, int batc
 enum lfm_kv_format { LFM_KV_F32 = 0, LFM_KV_BF16 = 1, LFM_KV_INT8 = 2, LFM_KV_FP8 = 3 };
 
 /* The caller's cache buffers: k and v [num_pages][kv_heads][page_tokens][64] of
- * the format's type, 16-byte aligned; k_scale and v_scale [num_pages][kv_heads]
- * [page_tokens] fp32 for INT8 and FP8, NULL for the others.  page_tokens is a
+ * the format's type; k_scale and v_scale [num_pages][kv_heads][page_tokens] fp32
+ * for INT8 and FP8, NULL for the others; all 16-byte aligned.  page_tokens is a
  * power of two, 16 to 4096.  Nothing has to be initialised. */
 typedef struct lfm_kv_cache {
   int format;

@@ -262,7 +262,9 @@ def check(pool, q, x, heads, got, hide=None, skip=()):
     (numerator and sum), so an output by 2 d sum p|v|.  d: q's scaling and at most 64 sums
     round (66 steps of sum |q||k| / 8), and exp's argument, no larger than twice that plus
     the scores' spread, rounds twice.  Then N sums of p v, of p, a weight's and an output's
-    few roundings: N + 24 steps."""
+    few roundings: N + 24 steps.  fp32 has no weights below 2^-126 of the largest (they may
+    count as 0), nor products of a weight with a row's scale (a stored value is at most 448):
+    N 2^-126 max(|v|, 448) off at most, where the sum of weights is at least 1."""
     G = heads // pool.kv
     fk, fv = pool.get(q.front, q.prefix) if q.prefix else (np.zeros((0, pool.kv, 64), np.float32),) * 2
     worst = 0.0
@@ -279,7 +281,7 @@ def check(pool, q, x, heads, got, hide=None, skip=()):
             qr = x[q.rows(b), h * 64:(h + 1) * 64]
             ref, mag, size = R.attention(qr, k[:, h // G], v[:, h // G], vis)
             d = (66 + 4) * EPS * size + 4 * EPS
-            tol = (2 * d[:, None] + (len(k) + 24) * EPS) * mag + 2.0 ** -120
+            tol = (2 * d[:, None] + (len(k) + 24) * EPS) * mag + len(k) * 2.0 ** -126 * max(448.0, np.abs(v[:, h // G]).max())
             err = np.abs(got[q.rows(b), h * 64:(h + 1) * 64] - ref)
             assert (err <= tol).all(), (b, h, float((err / tol).max()))
             worst = max(worst, float((err / np.maximum(tol, 1e-300)).max(initial=0.0)))

@@ -44,7 +44,7 @@ def attend(lib, c, b, q=A, ld=48 * 64, out=2 * A, ldo=32 * 64, heads=32, ws=A, n
 
 BAD_CACHES = [(dict(format=4), 2), (dict(format=-1), 2), (dict(kv_heads=0), 1), (dict(kv_heads=257), 2),
               (dict(page_tokens=8), 2), (dict(page_tokens=24), 2), (dict(page_tokens=8192), 2), (dict(page_tokens=0), 1),
-              (dict(num_pages=0), 1), (dict(k=None), 1), (dict(v=A + 8), 1), (dict(k_scale=None), 1),
+              (dict(num_pages=0), 1), (dict(k=None), 1), (dict(v=A + 8), 1), (dict(k_scale=None), 1), (dict(v_scale=A + 4), 1),
               (dict(format=0), 1), (dict(format=1, k_scale=None), 1)]
 BAD_BATCHES = [(dict(batch=-1), 1), (dict(tokens=5), 1), (dict(max_new=-1), 1), (dict(own_len=None), 1),
                (dict(pages=None), 1), (dict(prefix_len=1), 1), (dict(prefix_len=-1), 1), (dict(max_len=-1), 1),
