@@ -132,6 +132,7 @@ constexpr int kFlashWaves = 4;
 constexpr int kFlashThreads = 64 * kFlashWaves;
 constexpr int kMinTiles = 8;        // tiles of a split, at least
 constexpr float kRaise = 8.0f;      // log2
+constexpr int kFewCols = 4;         // columns of a kernel whose 16 hold four columns' three parts
 constexpr int kJoinPitch = 68;      // floats per column of the joined O
 constexpr float kNoScore = -__builtin_inff();
 
@@ -149,6 +150,13 @@ struct FlashArgs {
 __host__ __device__ inline int part_tiles(int n, int parts) {
   const int tiles = (n + kKeys - 1) / kKeys, per = (tiles + parts - 1) / parts;
   return (max(per, kMinTiles) + kFlashWaves - 1) / kFlashWaves * kFlashWaves;
+}
+
+// What a part's sums (maximum, sum of weights) count under the maximum of all:
+// without a score as they are, 0 or NaN.
+__device__ __forceinline__ float part_scale(float2 part, float mx) {
+  if (part.x == kNoScore) return part.y == 0.0f ? 0.0f : 1.0f;
+  return __builtin_amdgcn_exp2f(part.x - mx);
 }
 
 // Keys and values of a tile as they were loaded.
@@ -214,32 +222,68 @@ __device__ __forceinline__ void split8_exact(const float (&x)[8], bf16x8 (&part)
   for (int q = 0; q < 3; ++q) part[q] = __builtin_bit_cast(bf16x8, p[q]);
 }
 
-// acc += the product of an operand of NP parts with one of three.
-template <int NP>
-__device__ __forceinline__ f32x4 mfma_parts(const bf16x8 (&x)[NP], const bf16x8 (&y)[3], f32x4 acc) {
-  if constexpr (NP == 1) {
+// One of these parts (0, 1, 2; zeros for 3).
+__device__ __forceinline__ bf16x8 part8(const float (&x)[8], int which) {
+  const uint32_t m1 = which == 0 ? 0u : which == 3 ? 0xFFFFFFFFu : 0xFFFF0000u, m2 = which == 2 ? 0xFFFF0000u : 0u;
+  u32x4 p;
 #pragma unroll
-    for (int q = 2; q >= 0; --q) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[0], y[q], acc, 0, 0, 0);
-  } else {
+  for (int j = 0; j < 4; ++j) {
+    uint32_t w[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const float v = x[2 * j + e], a = v - __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, v) & m1);
+      const float b = a - __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, a) & m2);
+      w[e] = __builtin_bit_cast(uint32_t, b);
+    }
+    p[j] = pack_hi(w[0], w[1]);
+  }
+  return __builtin_bit_cast(bf16x8, p);
+}
+
+// Sum over the four columns c, c ^ 4, ... of a row of 16 lanes.
+__device__ __forceinline__ float sum_parts(float v) {
+  v += __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0x128, 0xf, 0xf, true));
+  return v + __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0x124, 0xf, 0xf, true));
+}
+
+// acc += the product of an operand of NP parts with one of QP: the six largest
+// products of three parts by three; where one side has one part, all.
+template <size_t NP, size_t QP>
+__device__ __forceinline__ f32x4 mfma_parts(const bf16x8 (&x)[NP], const bf16x8 (&y)[QP], f32x4 acc) {
+  if constexpr (NP == 3 && QP == 3) {
 #pragma unroll
     for (int m = 0; m < moe::kSplitProducts; ++m)
       acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[moe::kSplitA[m]], y[moe::kSplitB[m]], acc, 0, 0, 0);
+  } else {
+#pragma unroll
+    for (int n = (int)(NP * QP) - 1; n >= 0; --n)
+      acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[NP == 1 ? 0 : n], y[QP == 1 ? 0 : n], acc, 0, 0, 0);
   }
   return acc;
 }
 
+constexpr int flash_waves(int fmt, int ct) {
+  return fmt == LFM_KV_F32 ? 2 : ct == 0 ? 4 : ct == 1 ? 3 : 2;
+}
+
 template <int FMT, int CT, bool PREFIX>
-__global__ __launch_bounds__(kFlashThreads) __attribute__((amdgpu_waves_per_eu(CT == 1 ? 3 : 2)))
+__global__ __launch_bounds__(kFlashThreads) __attribute__((amdgpu_waves_per_eu(flash_waves(FMT, CT))))
 void kv_flash_kernel(KvArgs a, FlashArgs f) {
   using Raw = RawTile<FMT>;
   constexpr int NP = FMT == LFM_KV_F32 ? 3 : 1;
-  __shared__ float s_o[kFlashWaves][CT * 16 * kJoinPitch];
-  __shared__ float2 s_m[kFlashWaves][CT * 16];
+  // q's parts as operands [column tile][k-step][part][lane], then the waves' sums
+  constexpr bool FEW = CT == 0;
+  constexpr int NT = FEW ? 1 : CT, COLS = FEW ? kFewCols : 16 * CT, QP = FEW ? 1 : 3;
+  constexpr int kSumFloats = kFlashWaves * COLS * kJoinPitch, kPartFloats = NT * 2 * QP * 64 * 4;
+  __shared__ float s_lds[kSumFloats > kPartFloats ? kSumFloats : kPartFloats];
+  __shared__ float2 s_m[kFlashWaves][COLS];
+  bf16x8 *const s_q = reinterpret_cast<bf16x8 *>(s_lds);
   const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   // kv head fastest: with 8 of them a head's keys stay in one XCD's L2
   const int h = blockIdx.x % a.kv_heads, part = blockIdx.x / a.kv_heads;
-  const int col0 = blockIdx.y * CT * 16;
+  const int col0 = blockIdx.y * COLS;
+  const int lc = FEW ? c & 3 : c;  // the lane's column in its tile
 
   KvSeq s;
   const int *table;
@@ -260,52 +304,68 @@ void kv_flash_kernel(KvArgs a, FlashArgs f) {
   if (part * per * kKeys >= len) return;
   const bool direct = !PREFIX && f.prefix_parts == 0 && per * kKeys >= len;
   // the last position a column of the block sees
-  const int seen = PREFIX ? len : min(len, len - s.n + (col0 + CT * 16 - 1) / f.group + 1);
+  const int seen = PREFIX ? len : min(len, len - s.n + (col0 + COLS - 1) / f.group + 1);
   const int t_end = min((part + 1) * per, (seen + kKeys - 1) / kKeys);
 
-  // q's parts, scaled so that a score is the log2 of its weight
-  bf16x8 qp[CT][2][3];
-  int last[CT];  // last position the lane's columns see
+  // Pages of the wave's next 32 tiles, a half tile's in each lane (-1 outside the cache).
+  const int t0 = part * per + wave;
+  int pages = 0;
+  auto find_pages = [&](int t) {
+    const int k0 = min((t + kFlashWaves * (lane >> 1)) * kKeys + 16 * (lane & 1), (len - 1) & ~15);
+    pages = table[k0 >> a.pshift];
+    if (pages < 0 || pages >= a.num_pages) {
+      kv_flag(a.bad);
+      pages = -1;
+    }
+  };
+  find_pages(t0);
+
+  // q's parts, scaled so that a score is the log2 of its weight; wave w prepares
+  // the column tiles' k-steps w, w + 4, ...
+  int last[NT];  // last position the lane's columns see
 #pragma unroll
-  for (int ct = 0; ct < CT; ++ct) {
-    const int col = col0 + ct * 16 + c, tok = col / f.group, qh = h * f.group + col - tok * f.group;
+  for (int ct = 0; ct < NT; ++ct) last[ct] = PREFIX ? len - 1 : len - s.n + (col0 + ct * 16 + lc) / f.group;
+  for (int e = wave; e < 2 * NT; e += kFlashWaves) {
+    const int ct = e >> 1, st = e & 1;
+    const int col = col0 + ct * 16 + lc, tok = col / f.group, qh = h * f.group + col - tok * f.group;
     const bool valid = tok < s.n;
-    last[ct] = PREFIX ? len - 1 : len - s.n + tok;
     const float *qr = f.q + (size_t)(s.row0 + (valid ? tok : 0)) * f.ld + qh * kRowDim;
+    float x[8];
 #pragma unroll
-    for (int st = 0; st < 2; ++st) {
-      float x[8];
+    for (int j = 0; j < 8; j += 4) {
+      const f32x4 v = moe::ld4(qr + key_dim<FMT>(st, g, j));
 #pragma unroll
-      for (int j = 0; j < 8; j += 4) {
-        const f32x4 v = moe::ld4(qr + key_dim<FMT>(st, g, j));
+      for (int i = 0; i < 4; ++i) x[j + i] = valid ? v[i] * (0.125f * 1.44269504088896340736f) : 0.0f;
+    }
+    if constexpr (FEW) {
+      s_q[e * 64 + lane] = part8(x, c >> 2);
+    } else {
+      bf16x8 part3[3];
+      split8_exact(x, part3);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[j + e] = valid ? v[e] * (0.125f * 1.44269504088896340736f) : 0.0f;
-      }
-      split8_exact(x, qp[ct][st]);
+      for (int q = 0; q < 3; ++q) s_q[(e * 3 + q) * 64 + lane] = part3[q];
     }
   }
 
-  f32x4 o[CT][4];
-  float m[CT], l[CT];
+  f32x4 o[NT][4];
+  float m[NT], l[NT];
 #pragma unroll
-  for (int ct = 0; ct < CT; ++ct) {
+  for (int ct = 0; ct < NT; ++ct) {
     m[ct] = kNoScore;
     l[ct] = 0.0f;
 #pragma unroll
     for (int d = 0; d < 4; ++d) o[ct][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   }
 
-  auto load = [&](int t, Raw &r) {
+  auto load = [&](int n, Raw &r) {  // the wave's n-th tile
+    const int t = t0 + n * kFlashWaves;
+    if (n > 0 && (n & 31) == 0) find_pages(t);
 #pragma unroll
     for (int hb = 0; hb < 2; ++hb) {
       const int k0 = min(t * kKeys + 16 * hb, (len - 1) & ~15);
-      int page = __builtin_amdgcn_readfirstlane(table[k0 >> a.pshift]);
-      r.ok[hb] = page >= 0 && page < a.num_pages;
-      if (!r.ok[hb]) {
-        kv_flag(a.bad);
-        page = 0;
-      }
-      const size_t row = kv_row(a, page, h, k0 & ((1 << a.pshift) - 1));
+      const int page = __builtin_amdgcn_readlane(pages, 2 * (n & 31) + hb);
+      r.ok[hb] = page >= 0;
+      const size_t row = kv_row(a, max(page, 0), h, k0 & ((1 << a.pshift) - 1));
       const char *kp = a.k + row * kRowDim * kv_size<FMT>(), *vp = a.v + row * kRowDim * kv_size<FMT>();
 #pragma unroll
       for (int w = 0; w < Raw::KW; ++w)
@@ -439,13 +499,20 @@ void kv_flash_kernel(KvArgs a, FlashArgs f) {
     }
 
 #pragma unroll
-    for (int ct = 0; ct < CT; ++ct) {
+    for (int ct = 0; ct < NT; ++ct) {
       float p[8];  // scores, then weights, of keys 16 hb + 4g + i
+      bf16x8 qp[2][QP];
+#pragma unroll
+      for (int e = 0; e < 2 * QP; ++e) qp[e / QP][e % QP] = s_q[(ct * 2 * QP + e) * 64 + lane];
 #pragma unroll
       for (int hb = 0; hb < 2; ++hb) {
         f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int st = 0; st < 2; ++st) acc = mfma_parts<NP>(kop[hb][st], qp[ct][st], acc);
+        for (int st = 0; st < 2; ++st) acc = mfma_parts(kop[hb][st], qp[st], acc);
+        if constexpr (FEW) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[i] = sum_parts(acc[i]);
+        }
         if constexpr (Raw::SCALED) acc *= r.ks[hb];
 #pragma unroll
         for (int i = 0; i < 4; ++i) p[4 * hb + i] = acc[i];
@@ -483,10 +550,13 @@ void kv_flash_kernel(KvArgs a, FlashArgs f) {
             if (!r.ok[e >> 2] || k0 + 16 * (e >> 2) + 4 * g + (e & 3) > last[ct]) p[e] = 0.0f;
         }
       }
-      bf16x8 pp[3];
-      split8_exact(p, pp);
+      bf16x8 pp[QP];
+      if constexpr (FEW)
+        pp[0] = part8(p, c >> 2);
+      else
+        split8_exact(p, pp);
 #pragma unroll
-      for (int d = 0; d < 4; ++d) o[ct][d] = mfma_parts<NP>(vop[d], pp, o[ct][d]);
+      for (int d = 0; d < 4; ++d) o[ct][d] = mfma_parts(vop[d], pp, o[ct][d]);
       if (apart) {
         // how many of them a column sees: a product of ones
         u32x4 see;
@@ -510,40 +580,44 @@ void kv_flash_kernel(KvArgs a, FlashArgs f) {
     }
   };
 
-  // Two tiles in registers: one computed, one on its way.  A load past the
+  // Two tiles in registers: one computed, one on its way.  The load past the
   // wave's last tile repeats that one (its lines are in L2).
-  const int t0 = part * per + wave;
-  if (t0 < t_end) {
-    Raw ra, rb;
-    const int t_last = t0 + (t_end - 1 - t0) / kFlashWaves * kFlashWaves;
-    load(t0, ra);
-    for (int t = t0; t < t_end; t += 2 * kFlashWaves) {
-      load(min(t + kFlashWaves, t_last), rb);
-      compute(t, ra);
-      if (t + kFlashWaves >= t_end) break;
-      load(min(t + 2 * kFlashWaves, t_last), ra);
-      compute(t + kFlashWaves, rb);
-    }
+  Raw ra, rb;
+  if (t0 < t_end) load(0, ra);
+  __syncthreads();  // q's parts are there
+  for (int t = t0, n = 0; t < t_end; t += kFlashWaves, ++n) {
+    load(t + kFlashWaves < t_end ? n + 1 : n, rb);
+    compute(t, ra);
+    ra = rb;
   }
+  __syncthreads();  // and read for the last time
 
   // Join the waves: a common maximum, then sums.  O^T row 4g + i of block db is
   // dimension 16g + 4i + db.
 #pragma unroll
-  for (int ct = 0; ct < CT; ++ct) {
+  for (int ct = 0; ct < NT; ++ct) {
     l[ct] += __shfl_xor(l[ct], 16);
     l[ct] += __shfl_xor(l[ct], 32);
-    if (g == 0) s_m[wave][ct * 16 + c] = float2{m[ct], l[ct]};
+    if (FEW) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      moe::st4(&s_o[wave][(ct * 16 + c) * kJoinPitch + 16 * g + 4 * i],
-               f32x4{o[ct][0][i], o[ct][1][i], o[ct][2][i], o[ct][3][i]});
+      for (int d = 0; d < 4; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[ct][d][i] = sum_parts(o[ct][d][i]);
+    }
+    if (c < COLS) {
+      if (g == 0) s_m[wave][ct * 16 + c] = float2{m[ct], l[ct]};
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        moe::st4(&s_lds[(wave * COLS + ct * 16 + c) * kJoinPitch + 16 * g + 4 * i],
+                 f32x4{o[ct][0][i], o[ct][1][i], o[ct][2][i], o[ct][3][i]});
+    }
   }
   __syncthreads();
 #pragma unroll
-  for (int n = 0; n < CT; ++n) {
+  for (int n = 0; n < NT; ++n) {
     const int e = n * kFlashThreads + threadIdx.x, cc = e >> 4, d = (e & 15) * 4;
     const int col = col0 + cc, tok = col / f.group, qh = h * f.group + col - tok * f.group;
-    if (tok >= s.n) continue;
+    if (cc >= COLS || tok >= s.n) continue;
     float mw[kFlashWaves], mx = kNoScore, lt = 0.0f;
 #pragma unroll
     for (int w = 0; w < kFlashWaves; ++w) {
@@ -553,13 +627,14 @@ void kv_flash_kernel(KvArgs a, FlashArgs f) {
     f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int w = 0; w < kFlashWaves; ++w) {
-      const float sc = mw[w] == kNoScore ? (s_m[w][cc].y == 0.0f ? 0.0f : 1.0f) : __builtin_amdgcn_exp2f(mw[w] - mx);
+      const float sc = part_scale(float2{mw[w], s_m[w][cc].y}, mx);
       lt += s_m[w][cc].y * sc;
-      v += moe::ld4(&s_o[w][cc * kJoinPitch + d]) * sc;
+      v += moe::ld4(&s_lds[(w * COLS + cc) * kJoinPitch + d]) * sc;
     }
     const size_t row = (size_t)(s.row0 + tok) * f.heads + qh;
     if (direct) {
-      moe::st4(f.out + (size_t)(s.row0 + tok) * f.ldo + qh * kRowDim + d, lt == 0.0f ? v * 0.0f : v * (1.0f / lt));
+      moe::st4(f.out + (size_t)(s.row0 + tok) * f.ldo + qh * kRowDim + d,
+               lt == 0.0f ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : v * (1.0f / lt));
     } else {
       const size_t at = (size_t)(PREFIX ? f.own_parts + part : part) * f.rows + row;
       moe::st4(f.po + at * kRowDim + d, v);
@@ -568,33 +643,55 @@ void kv_flash_kernel(KvArgs a, FlashArgs f) {
   }
 }
 
-// Joins the parts of a token's head: one wave per row, a lane a dimension.
+// Joins the parts of a token's head, a wave per row: 16 lanes take a part's 64
+// sums, so four parts are loaded at a time, and a lane a part's maximum.
 __global__ __launch_bounds__(256) void kv_join_kernel(KvArgs a, FlashArgs f) {
   KvSeq s;
   if (!kv_seq<true>(a, blockIdx.y, s)) return;
   const int r = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
   if (r >= s.n * f.heads) return;
   const int own_per = part_tiles(s.len, f.own_parts) * kKeys, own = (s.len + own_per - 1) / own_per;
-  int pre = 0;
+  int parts = own;
   if (f.prefix_parts > 0) {
     const int per = part_tiles(a.prefix_len, f.prefix_parts) * kKeys;
-    pre = (a.prefix_len + per - 1) / per;
+    parts += (a.prefix_len + per - 1) / per;
   } else if (own == 1) {
     return;  // written by its one block
   }
   const size_t row = (size_t)s.row0 * f.heads + r;
   const int tok = r / f.heads, qh = r - tok * f.heads;
   auto at = [&](int p) { return (size_t)(p < own ? p : f.own_parts + p - own) * f.rows + row; };
-  float mx = kNoScore;
-  for (int p = 0; p < own + pre; ++p) mx = fmaxf(mx, f.pm[at(p)].x);
-  float lt = 0.0f, v = 0.0f;
-  for (int p = 0; p < own + pre; ++p) {
-    const float2 ml = f.pm[at(p)];
-    const float sc = ml.x == kNoScore ? (ml.y == 0.0f ? 0.0f : 1.0f) : __builtin_amdgcn_exp2f(ml.x - mx);
-    lt += ml.y * sc;
-    v += f.po[at(p) * kRowDim + lane] * sc;
+  float mx = kNoScore, lt = 0.0f;
+  f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (int p0 = 0; p0 < parts; p0 += 64) {
+    float2 ml = {kNoScore, 0.0f};
+    if (p0 + lane < parts) ml = f.pm[at(p0 + lane)];
+    float mn = ml.x;
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) mn = fmaxf(mn, __shfl_xor(mn, d));
+    mn = fmaxf(mn, mx);
+    const float old = part_scale(float2{mx, lt}, mn), sc = part_scale(ml, mn);
+    mx = mn;
+    float sum = ml.y * sc;
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) sum += __shfl_xor(sum, d);
+    lt = lt * old + sum;
+    v *= old;
+    const int n = min(parts - p0, 64);
+    for (int p = 0; p < n; p += 4) {
+      const int mine = p + (lane >> 4);
+      const float w = __shfl(sc, mine & 63);
+      if (mine < n) v += moe::ld4(f.po + at(p0 + mine) * kRowDim + (lane & 15) * 4) * w;
+    }
   }
-  f.out[(size_t)(s.row0 + tok) * f.ldo + qh * kRowDim + lane] = lt == 0.0f ? 0.0f : v * (1.0f / lt);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[i] += __shfl_xor(v[i], 16);
+    v[i] += __shfl_xor(v[i], 32);
+  }
+  if (lane < 16)
+    moe::st4(f.out + (size_t)(s.row0 + tok) * f.ldo + qh * kRowDim + lane * 4,
+             lt == 0.0f ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : v * (1.0f / lt));
 }
 
 // ---------------------------------------------------------------------------
@@ -641,17 +738,20 @@ hipError_t launch_kv_read(const KvArgs &a, float *k_out, float *v_out, int rows,
 
 // How a call is split: column tiles a wave holds, and parts of the own positions
 // and of the prefix so that about kFlashBlocks blocks run.
-constexpr int kFlashBlocks = 1024;
+constexpr int kFlashBlocks = 1024, kWideBlocks = 512;
 
 struct FlashPlan {
   int own_ct, prefix_ct, own_groups, prefix_groups, own_parts, prefix_parts;
 };
 
-static int column_tiles(long long cols) { return cols <= 16 ? 1 : cols <= 32 ? 2 : 4; }
+static int column_tiles(long long cols) { return cols <= kFewCols ? 0 : cols <= 16 ? 1 : cols <= 32 ? 2 : 4; }
 
-static int parts_of(long long keys, long long blocks) {
+static int columns_of(int ct) { return ct == 0 ? kFewCols : 16 * ct; }
+
+static int parts_of(long long keys, long long blocks, int ct) {
   const long long tiles = (keys + kKeys - 1) / kKeys, most = std::max<long long>(1, tiles / kMinTiles);
-  return (int)std::min<long long>({most, std::max<long long>(1, (kFlashBlocks + blocks - 1) / blocks), 256});
+  const long long want = ct <= 1 ? kFlashBlocks : kWideBlocks;
+  return (int)std::min<long long>({most, std::max<long long>(1, (want + blocks - 1) / blocks), 256});
 }
 
 static FlashPlan flash_plan(const KvArgs &a, int heads) {
@@ -659,13 +759,13 @@ static FlashPlan flash_plan(const KvArgs &a, int heads) {
   const long long group = heads / a.kv_heads, cap = (long long)a.max_pages << a.pshift;
   const int widest = a.format == LFM_KV_F32 ? 2 : 4;
   p.own_ct = std::min(widest, column_tiles(a.max_new * group));
-  p.own_groups = (int)((a.max_new * group + 16 * p.own_ct - 1) / (16 * p.own_ct));
+  p.own_groups = (int)((a.max_new * group + columns_of(p.own_ct) - 1) / columns_of(p.own_ct));
   p.own_parts = parts_of(std::min<long long>(a.max_len ? a.max_len : cap, cap),
-                         (long long)p.own_groups * a.kv_heads * std::max(a.batch, 1));
+                         (long long)p.own_groups * a.kv_heads * std::max(a.batch, 1), p.own_ct);
   if (a.prefix_len > 0) {
     p.prefix_ct = std::min(widest, column_tiles(a.tokens * group));
-    p.prefix_groups = (int)((a.tokens * group + 16 * p.prefix_ct - 1) / (16 * p.prefix_ct));
-    p.prefix_parts = parts_of(a.prefix_len, (long long)p.prefix_groups * a.kv_heads);
+    p.prefix_groups = (int)((a.tokens * group + columns_of(p.prefix_ct) - 1) / columns_of(p.prefix_ct));
+    p.prefix_parts = parts_of(a.prefix_len, (long long)p.prefix_groups * a.kv_heads, p.prefix_ct);
   }
   return p;
 }
@@ -681,6 +781,7 @@ size_t kv_attention_ws(const KvArgs &a, int heads) {
 template <int FMT, bool PREFIX>
 static hipError_t kv_flash_launch(const KvArgs &a, const FlashArgs &f, int ct, dim3 grid, hipStream_t st) {
   switch (ct) {
+    case 0: hipLaunchKernelGGL((kv_flash_kernel<FMT, 0, PREFIX>), grid, dim3(kFlashThreads), 0, st, a, f); break;
     case 1: hipLaunchKernelGGL((kv_flash_kernel<FMT, 1, PREFIX>), grid, dim3(kFlashThreads), 0, st, a, f); break;
     case 2: hipLaunchKernelGGL((kv_flash_kernel<FMT, 2, PREFIX>), grid, dim3(kFlashThreads), 0, st, a, f); break;
     default:
