@@ -1,107 +1,445 @@
 // HIP kernels from logits to tokens (gfx950): softmax with a temperature, and
 // verification of drafted tokens against the target's probabilities.
+#include <algorithm>
+
 #include "gpu_common.h"
 #include "lfm_internal.h"
 
 namespace lfm {
 
+using moe::f32x4;
+
 // ---------------------------------------------------------------------------
 // Softmax
 // ---------------------------------------------------------------------------
+//
+// A row's maximum and its sum of exponentials under that maximum, in fp32, then
+// the quotients.  A thread keeps the values it loaded, so a row is read once
+// where a block takes a whole one; where that leaves CUs idle a row is split
+// over blocks that leave their maximum and sum in the workspace to a second
+// kernel, which reads the row again (from L2).  An exponential is 2 to the power of
+// the rounded difference times c = log2(e) / temperature: v_exp_f32 does it in one
+// instruction, where expf's 15 made a row's 65536 values 9 us of arithmetic.
 
 constexpr int kSoftThreads = 1024;
+constexpr int kSoftRegs = 64;        // values a thread keeps
+constexpr int kSoftRow = kSoftThreads * kSoftRegs;
+constexpr int kSliceThreads = 256;   // a slice of a split row
+constexpr int kSliceRegs = 16;
+constexpr int kSlice = kSliceThreads * kSliceRegs;
 
-template <typename F>
-__device__ __forceinline__ float block_fold(float v, float *s_part, F f) {
+struct MaxSum {
+  float m, l;
+};
+
+// What a sum under maximum `m` counts under `mx` (a part with nothing but
+// -infinity has sum 0, or NaN with a NaN in it).
+__device__ __forceinline__ float rescale(float m, float mx, float c) {
+  return m == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f((m - mx) * c);
+}
+
+__device__ __forceinline__ float wave_max(float v) {
 #pragma unroll
-  for (int d = 32; d > 0; d >>= 1) v = f(v, __shfl_xor(v, d));
-  __syncthreads();  // readers of the fold before this one are done
-  if ((threadIdx.x & 63) == 0) s_part[threadIdx.x >> 6] = v;
-  __syncthreads();
-  v = s_part[0];
-  for (int i = 1; i < kSoftThreads / 64; ++i) v = f(v, s_part[i]);
+  for (int d = 32; d > 0; d >>= 1) v = fmaxf(v, __shfl_xor(v, d));
   return v;
 }
 
-__global__ __launch_bounds__(kSoftThreads) void softmax_kernel(const float *x, long long xs, float *y, long long ys,
-                                                               int dim, float inv_t) {
-  __shared__ float s_part[kSoftThreads / 64];
-  x += blockIdx.x * xs;
-  y += blockIdx.x * ys;
-  float m = -__builtin_inff();
-  for (int i = threadIdx.x; i < dim; i += kSoftThreads) m = fmaxf(m, x[i]);
-  m = block_fold(m, s_part, [](float p, float q) { return fmaxf(p, q); });
-  if (m == -__builtin_inff()) m = 0.0f;
-  float l = 0.0f;
-  for (int i = threadIdx.x; i < dim; i += kSoftThreads) l += expf((x[i] - m) * inv_t);
-  l = block_fold(l, s_part, [](float p, float q) { return p + q; });
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  for (int i = threadIdx.x; i < dim; i += kSoftThreads) y[i] = expf((x[i] - m) * inv_t) * inv;
+__device__ __forceinline__ float wave_sum(float v) {
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d);
+  return v;
 }
 
-size_t softmax_ws(int, int) { return 0; }
+// Maximum over a block of NW waves, then the sum of exponentials: v becomes
+// exp((v - max) / t).  Values of -infinity give 0 whatever the maximum.
+template <int NW, int NR>
+__device__ __forceinline__ MaxSum block_exp(float (&v)[NR], float c, float *s_part) {
+  const int wave = threadIdx.x >> 6;
+  float m = -__builtin_inff();
+#pragma unroll
+  for (int j = 0; j < NR; ++j) m = fmaxf(m, v[j]);
+  m = wave_max(m);
+  if ((threadIdx.x & 63) == 0) s_part[wave] = m;
+  __syncthreads();
+  m = s_part[0];
+#pragma unroll
+  for (int w = 1; w < NW; ++w) m = fmaxf(m, s_part[w]);
+  const float ref = m == -__builtin_inff() ? 0.0f : m;
+  float l = 0.0f;
+#pragma unroll
+  for (int j = 0; j < NR; ++j) {
+    v[j] = __builtin_amdgcn_exp2f((v[j] - ref) * c);
+    l += v[j];
+  }
+  l = wave_sum(l);
+  if ((threadIdx.x & 63) == 0) s_part[NW + wave] = l;
+  __syncthreads();
+  l = s_part[NW];
+#pragma unroll
+  for (int w = 1; w < NW; ++w) l += s_part[NW + w];
+  return {m, l};
+}
+
+// Values [0, n) of x to registers, thread t's j-th group of VEC at (j * threads + t) * VEC;
+// -infinity behind them.
+template <int NW, int NR, int VEC>
+__device__ __forceinline__ void load_values(const float *x, int n, float (&v)[NR]) {
+#pragma unroll
+  for (int j = 0; j < NR / VEC; ++j) {
+    const int i = (j * NW * 64 + (int)threadIdx.x) * VEC;
+    if (VEC == 4) {  // n % 4 == 0
+      const f32x4 w = i < n ? moe::ld4(x + i) : f32x4(-__builtin_inff());
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[4 * j + e] = w[e];
+    } else {
+      v[j] = i < n ? x[i] : -__builtin_inff();
+    }
+  }
+}
+
+template <int NW, int NR, int VEC>
+__device__ __forceinline__ void store_values(float *y, int n, const float (&v)[NR], float scale) {
+#pragma unroll
+  for (int j = 0; j < NR / VEC; ++j) {
+    const int i = (j * NW * 64 + (int)threadIdx.x) * VEC;
+    if (i >= n) continue;
+    if (VEC == 4) {
+      moe::st4(y + i, f32x4{v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]} * scale);
+    } else {
+      y[i] = v[j] * scale;
+    }
+  }
+}
+
+__device__ __forceinline__ float inverse_sum(float l) { return l == 0.0f ? 0.0f : 1.0f / l; }
+
+// A row a block, NR values a thread.
+template <int NR, int VEC>
+__global__ __launch_bounds__(kSoftThreads) __attribute__((amdgpu_waves_per_eu(NR <= 32 ? 8 : 4)))
+void softmax_row_kernel(const float *x, long long xs, float *y, long long ys,
+                                                                   int dim, float c) {
+  constexpr int NW = kSoftThreads / 64;
+  __shared__ float s_part[2 * NW];
+  x += blockIdx.x * xs;
+  y += blockIdx.x * ys;
+  float v[NR];
+  load_values<NW, NR, VEC>(x, dim, v);
+  const MaxSum r = block_exp<NW, NR>(v, c, s_part);
+  store_values<NW, NR, VEC>(y, dim, v, inverse_sum(r.l));
+}
+
+// A slice of a row a block: its maximum and sum.
+template <int VEC>
+__global__ __launch_bounds__(kSliceThreads) void softmax_part_kernel(const float *x, long long xs, float2 *part, int dim,
+                                                                     float c) {
+  constexpr int NW = kSliceThreads / 64;
+  __shared__ float s_part[2 * NW];
+  const int first = blockIdx.x * kSlice, n = min(dim - first, kSlice);
+  float v[kSliceRegs];
+  load_values<NW, kSliceRegs, VEC>(x + blockIdx.y * xs + first, n, v);
+  const MaxSum r = block_exp<NW, kSliceRegs>(v, c, s_part);
+  if (threadIdx.x == 0) part[(size_t)blockIdx.y * gridDim.x + blockIdx.x] = float2{r.m, r.l};
+}
+
+template <int VEC>
+__global__ __launch_bounds__(kSliceThreads) void softmax_finish_kernel(const float *x, long long xs, float *y,
+                                                                       long long ys, const float2 *part, int dim,
+                                                                       float c) {
+  constexpr int NW = kSliceThreads / 64;
+  const int first = blockIdx.x * kSlice, n = min(dim - first, kSlice), lane = threadIdx.x & 63;
+  float v[kSliceRegs];
+  load_values<NW, kSliceRegs, VEC>(x + blockIdx.y * xs + first, n, v);
+  // every wave joins the row's parts by itself
+  const float2 *p = part + (size_t)blockIdx.y * gridDim.x;
+  float m = -__builtin_inff();
+  for (int i = lane; i < (int)gridDim.x; i += 64) m = fmaxf(m, p[i].x);
+  m = wave_max(m);
+  const float ref = m == -__builtin_inff() ? 0.0f : m;
+  float l = 0.0f;
+  for (int i = lane; i < (int)gridDim.x; i += 64) l += p[i].y * rescale(p[i].x, ref, c);
+  const float inv = inverse_sum(wave_sum(l));
+#pragma unroll
+  for (int j = 0; j < kSliceRegs; ++j) v[j] = __builtin_amdgcn_exp2f((v[j] - ref) * c);
+  store_values<NW, kSliceRegs, VEC>(y + blockIdx.y * ys + first, n, v, inv);
+}
+
+// How many of the first rows are taken whole.  Short ones all are (8192 values:
+// one launch, 5 us); of rows up to kSoftRow values, of which a CU holds one or
+// two, full rounds of the CUs and a last one that is kSoftMost of a round: a
+// round of 65536 values takes 27 us, kSoftMost of it split as long.
+constexpr int kShortRow = 8 * kSoftThreads, kSoftCUs = 256;
+
+static int whole_rows(int rows, int dim) {
+  if (dim <= kShortRow) return rows;
+  if (dim > kSoftRow) return 0;
+  const int round = dim <= 32 * kSoftThreads ? 2 * kSoftCUs : kSoftCUs, left = rows % round;
+  return left >= round / 4 * 3 ? rows : rows - left;
+}
+
+size_t softmax_ws(int rows, int dim) {
+  return (size_t)(rows - whole_rows(rows, dim)) * ((dim + kSlice - 1) / kSlice) * sizeof(float2);
+}
+
+template <int VEC>
+static hipError_t softmax_launch(const float *x, long long xs, float *y, long long ys, int rows, int dim, float c,
+                                 void *ws, hipStream_t st) {
+  const int whole = whole_rows(rows, dim);
+  if (whole > 0) {
+    if (dim <= 8 * kSoftThreads)
+      hipLaunchKernelGGL((softmax_row_kernel<8, VEC>), dim3(whole), dim3(kSoftThreads), 0, st, x, xs, y, ys, dim, c);
+    else if (dim <= 32 * kSoftThreads)
+      hipLaunchKernelGGL((softmax_row_kernel<32, VEC>), dim3(whole), dim3(kSoftThreads), 0, st, x, xs, y, ys, dim, c);
+    else
+      hipLaunchKernelGGL((softmax_row_kernel<64, VEC>), dim3(whole), dim3(kSoftThreads), 0, st, x, xs, y, ys, dim, c);
+  }
+  const int slices = (dim + kSlice - 1) / kSlice;
+  float2 *part = static_cast<float2 *>(ws);
+  for (int r0 = whole; r0 < rows; r0 += 65535) {  // rows a launch may have
+    const dim3 grid(slices, std::min(rows - r0, 65535));
+    float2 *p = part + (size_t)(r0 - whole) * slices;
+    hipLaunchKernelGGL((softmax_part_kernel<VEC>), grid, dim3(kSliceThreads), 0, st, x + r0 * xs, xs, p, dim, c);
+    hipLaunchKernelGGL((softmax_finish_kernel<VEC>), grid, dim3(kSliceThreads), 0, st, x + r0 * xs, xs, y + r0 * ys, ys, p,
+                       dim, c);
+  }
+  return hipGetLastError();
+}
 
 hipError_t launch_softmax(const float *x, long long xs, float *y, long long ys, int rows, int dim,
-                          float temperature, void *, hipStream_t st) {
-  hipLaunchKernelGGL(softmax_kernel, dim3(rows), dim3(kSoftThreads), 0, st, x, xs, y, ys, dim, 1.0f / temperature);
-  return hipGetLastError();
+                          float temperature, void *ws, hipStream_t st) {
+  const float c = (float)(1.4426950408889634 / (double)temperature);
+  const bool wide = ((uintptr_t)x & 15u) == 0 && ((uintptr_t)y & 15u) == 0 && xs % 4 == 0 && ys % 4 == 0 && dim % 4 == 0;
+  return wide ? softmax_launch<4>(x, xs, y, ys, rows, dim, c, ws, st)
+              : softmax_launch<1>(x, xs, y, ys, rows, dim, c, ws, st);
 }
 
 // ---------------------------------------------------------------------------
 // Verification of drafted tokens
 // ---------------------------------------------------------------------------
+//
+// Only the row that a token is drawn from is read, and the draft's at a
+// rejection.  Sums are 64-bit, so that which id a random number falls on does
+// not hang on their order: a slice of kDrawSlice weights a block leaves two
+// sums (of the weights after a rejection, and of the target alone, for where
+// those have no positive sum), and a second kernel finds the slice, then the id
+// in it.  Every block of the first decides by itself which row that is.
 
-// Accepted drafts of sequence b (one thread's work; exact: a product of two
-// fp32 values is exact in 64 bits).
-__device__ inline int accepted_drafts(const VerifyArgs &a, int b, int n) {
-  for (int i = 0; i < n; ++i) {
-    const int id = a.ids[(size_t)b * a.n_draft + i];
-    if (id < 0 || id >= a.vocab) return i;
-    const float q = a.draft[((size_t)b * a.n_draft + i) * a.vocab + id];
-    const float p = a.target[((size_t)b * (a.n_draft + 1) + i) * a.vocab + id];
-    if (!((double)a.u_accept[(size_t)b * a.n_draft + i] * (double)q < (double)p)) return i;
+constexpr int kDrawThreads = 256;
+constexpr int kDrawRegs = 8;
+constexpr int kDrawSlice = kDrawThreads * kDrawRegs;
+
+// Accepted drafts of sequence b, found by one wave, 64 drafts at a time (exact:
+// a product of two fp32 values is exact in 64 bits).
+__device__ __forceinline__ int accepted_drafts(const VerifyArgs &a, int b, int n) {
+  const int lane = threadIdx.x & 63;
+  for (int i0 = 0; i0 < a.n_draft; i0 += 64) {
+    const int i = i0 + lane;
+    bool ok = i < a.n_draft;
+    if (ok) {
+      const size_t at = (size_t)b * a.n_draft + i;
+      const int id = a.ids[at];
+      const float u = a.u_accept[at];
+      ok = id >= 0 && id < a.vocab;
+      if (ok) {
+        const float q = a.draft[at * a.vocab + id];
+        const float p = a.target[(at + b) * a.vocab + id];  // [b][n_draft + 1]
+        ok = (double)u * (double)q < (double)p;
+      }
+    }
+    const unsigned long long no = __ballot(!ok);
+    if (no) return min(i0 + __builtin_ctzll(no), n);
   }
   return n;
 }
 
-// max(p - q, 0) in 64 bits, where the difference of two fp32 values of like
-// size is exact; NaN counts as 0.
+// max(p - q, 0); NaN counts as 0.
 __device__ __forceinline__ double weight(float p, float q) {
   const double d = (double)p - (double)q;
   return d > 0.0 ? d : 0.0;
 }
 
-// One thread per sequence.
-__global__ __launch_bounds__(64) void verify_kernel(VerifyArgs a) {
-  const int b = blockIdx.x * 64 + threadIdx.x;
-  if (b >= a.batch) return;
-  const int n = a.n_valid ? min(max(a.n_valid[b], 0), a.n_draft) : a.n_draft;
-  const int acc = accepted_drafts(a, b, n);
-  const float *p = a.target + ((size_t)b * (a.n_draft + 1) + acc) * a.vocab;
-  const float *q = acc < n ? a.draft + ((size_t)b * a.n_draft + acc) * a.vocab : nullptr;
-  double total = 0.0;
-  for (int v = 0; v < a.vocab; ++v) total += weight(p[v], q ? q[v] : 0.0f);
-  if (q && !(total > 0.0)) {
-    q = nullptr;
-    total = 0.0;
-    for (int v = 0; v < a.vocab; ++v) total += weight(p[v], 0.0f);
-  }
-  const double bar = (double)a.u_sample[b] * total;
-  int token = -1;
-  double sum = 0.0;
-  for (int v = 0; v < a.vocab && token < 0; ++v) {
-    sum += weight(p[v], q ? q[v] : 0.0f);
-    if (sum > bar) token = v;
-  }
-  a.accepted[b] = acc;
-  for (int i = 0; i <= a.n_draft; ++i)
-    a.tokens[(size_t)b * (a.n_draft + 1) + i] = i < acc ? a.ids[(size_t)b * a.n_draft + i] : i == acc ? token : -1;
+struct DrawRow {
+  const float *p, *q;  // q null: the target alone
+};
+
+__device__ __forceinline__ int drafts_of(const VerifyArgs &a, int b) {
+  return a.n_valid ? min(max(a.n_valid[b], 0), a.n_draft) : a.n_draft;
 }
 
-size_t verify_draft_ws(int, int) { return 0; }
+// The row that the token after `acc` accepted drafts is drawn from.
+__device__ __forceinline__ DrawRow row_after(const VerifyArgs &a, int b, int acc, int n) {
+  return {a.target + ((size_t)b * (a.n_draft + 1) + acc) * a.vocab,
+          acc < n ? a.draft + ((size_t)b * a.n_draft + acc) * a.vocab : nullptr};
+}
 
-hipError_t launch_verify_draft(const VerifyArgs &a, void *, hipStream_t st) {
-  hipLaunchKernelGGL(verify_kernel, dim3((a.batch + 63) / 64), dim3(64), 0, st, a);
+// Inclusive running sum over a wave, and its total: row shifts by 1, 2, 4, 8,
+// then the sums of a row of 16 and of the lower half broadcast upwards.  (DPP
+// moves of the two halves; shuffles through LDS took twice the kernel's time.)
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dpp_up(double v) {
+  const unsigned long long u = __builtin_bit_cast(unsigned long long, v);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, ROWS, 0xf, false);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, ROWS, 0xf, false);
+  return __builtin_bit_cast(double, (unsigned long long)hi << 32 | lo);
+}
+
+__device__ __forceinline__ double scan(double v) {
+  v += dpp_up<0x111, 0xf>(v);
+  v += dpp_up<0x112, 0xf>(v);
+  v += dpp_up<0x114, 0xf>(v);
+  v += dpp_up<0x118, 0xf>(v);
+  v += dpp_up<0x142, 0xa>(v);
+  return v + dpp_up<0x143, 0xc>(v);
+}
+
+__device__ __forceinline__ double lane_value(double v, int lane) {
+  const unsigned long long u = __builtin_bit_cast(unsigned long long, v);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)u, lane);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(u >> 32), lane);
+  return __builtin_bit_cast(double, (unsigned long long)hi << 32 | lo);
+}
+
+// Sum of one value of each thread, the same order in every thread.
+__device__ __forceinline__ double block_sum(double v, double *s_part) {
+  v = lane_value(scan(v), 63);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) s_part[threadIdx.x >> 6] = v;
+  __syncthreads();
+  v = s_part[0];
+#pragma unroll
+  for (int w = 1; w < kDrawThreads / 64; ++w) v += s_part[w];
+  return v;
+}
+
+__global__ __launch_bounds__(kDrawThreads) void draw_sums_kernel(VerifyArgs a, double2 *sums) {
+  __shared__ double s_part[kDrawThreads / 64];
+  const int b = blockIdx.y, first = blockIdx.x * kDrawSlice;
+  const int n = drafts_of(a, b);
+  const int acc = accepted_drafts(a, b, n);
+  const DrawRow r = row_after(a, b, acc, n);
+  if (blockIdx.x == 0 && threadIdx.x == 0) a.accepted[b] = acc;
+  double rest = 0.0, whole = 0.0;
+  const float *q = r.q ? r.q : r.p;
+  float pv[kDrawRegs], qv[kDrawRegs];  // every load without a branch: they are in flight together
+#pragma unroll
+  for (int j = 0; j < kDrawRegs; ++j) {
+    const int v = min(first + j * kDrawThreads + (int)threadIdx.x, a.vocab - 1);
+    pv[j] = r.p[v];
+    qv[j] = q[v];
+  }
+#pragma unroll
+  for (int j = 0; j < kDrawRegs; ++j) {
+    const bool there = first + j * kDrawThreads + (int)threadIdx.x < a.vocab;
+    whole += there ? weight(pv[j], 0.0f) : 0.0;
+    rest += there ? weight(pv[j], qv[j]) : 0.0;
+  }
+  whole = block_sum(whole, s_part);
+  if (r.q) rest = block_sum(rest, s_part);
+  if (threadIdx.x == 0) sums[(size_t)b * gridDim.x + blockIdx.x] = double2{rest, whole};
+}
+
+// The lowest id up to which the weights sum to more than u times their whole
+// sum; one block per sequence.  Every wave finds the slice, then each of the
+// 1024 threads takes two of its weights.  (With LDS atomics for the lowest id,
+// which the compiler turns into a loop over a wave's lanes, it took 8.5 us.)
+constexpr int kTokenThreads = 1024, kTokenRegs = kDrawSlice / kTokenThreads;
+
+__global__ __launch_bounds__(kTokenThreads) void draw_token_kernel(VerifyArgs a, const double2 *sums, int slices) {
+  __shared__ double s_part[kTokenThreads / 64];
+  __shared__ int s_token[kTokenThreads / 64], s_last[kTokenThreads / 64];
+  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
+  const int acc = a.accepted[b];
+  const float u = a.u_sample[b];
+  const int n = drafts_of(a, b);  // every load that hangs on nothing stands in front
+  const int id = tid < a.n_draft ? a.ids[(size_t)b * a.n_draft + tid] : -1;
+  sums += (size_t)b * slices;
+  // lane l holds the sums of `each` neighbouring slices
+  const int each = (slices + 63) / 64, i0 = lane * each, i1 = min(i0 + each, slices);
+  double rest = 0.0, whole = 0.0;
+  for (int i = i0; i < i1; ++i) {
+    rest += sums[i].x;
+    whole += sums[i].y;
+  }
+  const DrawRow r = row_after(a, b, acc, n);
+  bool use_rest = r.q != nullptr;
+  double mine = use_rest ? rest : whole, incl, total;
+  for (;;) {
+    incl = scan(mine);
+    total = lane_value(incl, 63);
+    if (!use_rest || total > 0.0) break;
+    use_rest = false;
+    mine = whole;
+  }
+  const double bar = (double)u * total;
+  const unsigned long long hit = __ballot(incl > bar && mine > 0.0);
+  int token = -1;
+  if (hit) {
+    const int at = __builtin_ctzll(hit);
+    double run = lane_value(incl - mine, at);
+    int slice = at * each;
+    for (int i = slice; i < min(slice + each, slices) - 1; ++i) {  // uniform
+      const double next = run + (use_rest ? sums[i].x : sums[i].y);
+      if (next > bar) break;
+      run = next;
+      ++slice;
+    }
+    const int v0 = slice * kDrawSlice + tid * kTokenRegs;
+    const float *q = r.q ? r.q : r.p;
+    float pv[kTokenRegs], qv[kTokenRegs];
+#pragma unroll
+    for (int j = 0; j < kTokenRegs; ++j) {
+      pv[j] = r.p[min(v0 + j, a.vocab - 1)];
+      qv[j] = q[min(v0 + j, a.vocab - 1)];
+    }
+    double w[kTokenRegs], sum = 0.0;
+#pragma unroll
+    for (int j = 0; j < kTokenRegs; ++j) {
+      w[j] = v0 + j < a.vocab ? weight(pv[j], use_rest ? qv[j] : 0.0f) : 0.0;
+      sum += w[j];
+    }
+    const double upto = scan(sum);
+    if (lane == 63) s_part[tid >> 6] = upto;
+    __syncthreads();
+    // a wave's first id past the bar and its last id of any weight, by lane order
+    const int wave = tid >> 6;
+    sum = run + (upto - sum);
+    for (int i = 0; i < wave; ++i) sum += s_part[i];
+    int past = -1, last = -1;
+#pragma unroll
+    for (int j = 0; j < kTokenRegs; ++j) {
+      sum += w[j];
+      if (w[j] > 0.0) {
+        last = v0 + j;
+        if (past < 0 && sum > bar) past = v0 + j;
+      }
+    }
+    const unsigned long long is_past = __ballot(past >= 0), is_last = __ballot(last >= 0);
+    const int first_past = is_past ? __builtin_amdgcn_readlane(past, __builtin_ctzll(is_past)) : -1;
+    const int at_last = is_last ? __builtin_amdgcn_readlane(last, 63 - __builtin_clzll(is_last)) : -1;
+    if (lane == 0) {
+      s_token[wave] = first_past;
+      s_last[wave] = at_last;
+    }
+    __syncthreads();
+    // the slice's sum was taken in another order: where only that passes the
+    // bar, the slice's last id it is
+    for (int i = kTokenThreads / 64 - 1; i >= 0; --i) token = max(token, s_last[i]);
+    for (int i = kTokenThreads / 64 - 1; i >= 0; --i)
+      if (s_token[i] >= 0) token = s_token[i];
+  }
+  int *out = a.tokens + (size_t)b * (a.n_draft + 1);
+  if (tid <= a.n_draft) out[tid] = tid < acc ? id : tid == acc ? token : -1;
+  if (tid == 0 && a.n_draft == kTokenThreads) out[a.n_draft] = acc == a.n_draft ? token : -1;
+}
+
+size_t verify_draft_ws(int batch, int vocab) {
+  return (size_t)batch * (((size_t)vocab + kDrawSlice - 1) / kDrawSlice) * sizeof(double2);
+}
+
+hipError_t launch_verify_draft(const VerifyArgs &a, void *ws, hipStream_t st) {
+  const int slices = (int)(((size_t)a.vocab + kDrawSlice - 1) / kDrawSlice);
+  double2 *sums = static_cast<double2 *>(ws);
+  hipLaunchKernelGGL(draw_sums_kernel, dim3(slices, a.batch), dim3(kDrawThreads), 0, st, a, sums);
+  hipLaunchKernelGGL(draw_token_kernel, dim3(a.batch), dim3(kTokenThreads), 0, st, a, sums, slices);
   return hipGetLastError();
 }
 
