@@ -3,6 +3,7 @@
 // read back, and attention of new tokens over a shared prefix and their own
 // pages.
 #include <algorithm>
+#include <type_traits>
 
 #include "lfm_kv.h"
 #include "lfm_rope.h"
@@ -122,14 +123,12 @@ __global__ __launch_bounds__(256) void kv_read_kernel(KvArgs a, float *k_out, fl
 //
 // The running maximum is only raised when a score passes it by kRaise: weights
 // then reach 2^kRaise, and most tiles need no exchange between lanes and no
-// scaling of O.
+// scaling of O.  A weight is 2 to the power of one FMA, score * scale - maximum.
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kKeys = 32;           // keys per tile
-constexpr int kFlashWaves = 4;
-constexpr int kFlashThreads = 64 * kFlashWaves;
 constexpr int kMinTiles = 8;        // tiles of a split, at least
 constexpr float kRaise = 8.0f;      // log2
 constexpr int kFewCols = 4;         // columns of a kernel whose 16 hold four columns' three parts
@@ -146,11 +145,25 @@ struct FlashArgs {
   size_t rows;                  // tokens * heads
 };
 
-// Tiles per part when `n` keys are split into at most `parts`.
-__host__ __device__ inline int part_tiles(int n, int parts) {
-  const int tiles = (n + kKeys - 1) / kKeys, per = (tiles + parts - 1) / parts;
-  return (max(per, kMinTiles) + kFlashWaves - 1) / kFlashWaves * kFlashWaves;
+// Parts that `keys` keys are split into, of at most `parts`.
+__host__ __device__ inline int active_parts(int keys, int parts) {
+  const int most = (keys + kKeys - 1) / kKeys / kMinTiles;
+  return most < 1 ? 1 : most < parts ? most : parts;
 }
+
+// Waves of a block: one token's few columns leave room, and time, for eight.
+__host__ __device__ constexpr int column_waves(int ct) { return ct == 0 ? 8 : 4; }
+
+// A block of W waves with CT tiles of 16 columns; CT = 0: kFewCols columns, whose
+// three parts fill a tile.
+template <int CT, int W>
+struct FlashShape {
+  static constexpr bool FEW = CT == 0;
+  static constexpr int NT = FEW ? 1 : CT, COLS = FEW ? kFewCols : 16 * CT, QP = FEW ? 1 : 3;
+  static constexpr int kSumFloats = W * COLS * kJoinPitch, kPartFloats = NT * 2 * QP * 64 * 4;
+  static constexpr int kFloats = kSumFloats > kPartFloats ? kSumFloats : kPartFloats;
+  static constexpr int kBytes = kFloats * 4 + W * COLS * 8;
+};
 
 // What a part's sums (maximum, sum of weights) count under the maximum of all:
 // without a score as they are, 0 or NaN.
@@ -203,26 +216,39 @@ __device__ __forceinline__ void widen4(uint32_t w, uint32_t &lo, uint32_t &hi) {
   }
 }
 
-// Three parts of eight floats, each exact in bf16 together (truncation: 8 bits a part).
+// x - the low (high) bf16 of a pair: exact where that is x rounded.  The factor
+// stands in a register: as an inline constant -1.0 the instruction takes it for
+// the upper half.
+__device__ __forceinline__ float less(float x, uint32_t pair, uint32_t minus_one) {
+  asm("" : "+s"(minus_one));
+  return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(kv_bf16x2, pair),
+                                         __builtin_bit_cast(kv_bf16x2, minus_one), x, false);
+}
+__device__ __forceinline__ float less_lo(float x, uint32_t pair) { return less(x, pair, 0xBF80u); }
+__device__ __forceinline__ float less_hi(float x, uint32_t pair) { return less(x, pair, 0xBF800000u); }
+__device__ __forceinline__ uint32_t round_pair(float lo, float hi) {
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(kv_f32x2{lo, hi}, kv_bf16x2));
+}
+
+// Three parts of eight floats, exact together: 8 bits each, rounded to nearest.
+// 28 instructions (the remainders by the bf16 dot product) where masks, subtractions
+// and byte permutes take 44.
 __device__ __forceinline__ void split8_exact(const float (&x)[8], bf16x8 (&part)[3]) {
   u32x4 p[3];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    uint32_t a0 = __builtin_bit_cast(uint32_t, x[2 * j]), b0 = __builtin_bit_cast(uint32_t, x[2 * j + 1]);
-    const float a1 = x[2 * j] - __builtin_bit_cast(float, a0 & 0xFFFF0000u);
-    const float b1 = x[2 * j + 1] - __builtin_bit_cast(float, b0 & 0xFFFF0000u);
-    const uint32_t ua = __builtin_bit_cast(uint32_t, a1), ub = __builtin_bit_cast(uint32_t, b1);
-    const float a2 = a1 - __builtin_bit_cast(float, ua & 0xFFFF0000u);
-    const float b2 = b1 - __builtin_bit_cast(float, ub & 0xFFFF0000u);
-    p[0][j] = pack_hi(a0, b0);
-    p[1][j] = pack_hi(ua, ub);
-    p[2][j] = byte_pair(a2, b2);
+    float a = x[2 * j], b = x[2 * j + 1];
+    p[0][j] = round_pair(a, b);
+    a = less_lo(a, p[0][j]);
+    b = less_hi(b, p[0][j]);
+    p[1][j] = round_pair(a, b);
+    p[2][j] = round_pair(less_lo(a, p[1][j]), less_hi(b, p[1][j]));
   }
 #pragma unroll
   for (int q = 0; q < 3; ++q) part[q] = __builtin_bit_cast(bf16x8, p[q]);
 }
 
-// One of these parts (0, 1, 2; zeros for 3).
+// One of three parts of eight floats (0, 1, 2; zeros for 3), 8 bits each, truncated.
 __device__ __forceinline__ bf16x8 part8(const float (&x)[8], int which) {
   const uint32_t m1 = which == 0 ? 0u : which == 3 ? 0xFFFFFFFFu : 0xFFFF0000u, m2 = which == 2 ? 0xFFFF0000u : 0u;
   u32x4 p;
@@ -262,108 +288,139 @@ __device__ __forceinline__ f32x4 mfma_parts(const bf16x8 (&x)[NP], const bf16x8 
   return acc;
 }
 
-constexpr int flash_waves(int fmt, int ct) {
-  return fmt == LFM_KV_F32 ? 2 : ct == 0 ? 4 : ct == 1 ? 3 : 2;
+// The operand of K for half tile hb and k-step st.
+template <int FMT, int NP>
+__device__ __forceinline__ void key_operand(const RawTile<FMT> &r, int hb, int st, bf16x8 (&op)[NP]) {
+  if constexpr (FMT == LFM_KV_F32) {
+    const f32x4 x[2] = {__builtin_bit_cast(f32x4, r.k[hb][2 * st]), __builtin_bit_cast(f32x4, r.k[hb][2 * st + 1])};
+    moe::split8(x, op);
+  } else if constexpr (FMT == LFM_KV_BF16) {
+    op[0] = __builtin_bit_cast(bf16x8, r.k[hb][st]);
+  } else {
+    uint32_t w[4];
+    widen4<FMT>(r.k[hb][0][2 * st], w[0], w[1]);
+    widen4<FMT>(r.k[hb][0][2 * st + 1], w[2], w[3]);
+    op[0] = __builtin_bit_cast(bf16x8, u32x4{w[0], w[1], w[2], w[3]});
+  }
 }
 
-template <int FMT, int CT, bool PREFIX>
-__global__ __launch_bounds__(kFlashThreads) __attribute__((amdgpu_waves_per_eu(flash_waves(FMT, CT))))
-void kv_flash_kernel(KvArgs a, FlashArgs f) {
+// The operands of V: block db takes dimension 4c + db of the lane's eight keys.
+template <int FMT, int NP>
+__device__ __forceinline__ void value_operands(const RawTile<FMT> &r, bf16x8 (&op)[4][NP]) {
+  if constexpr (FMT == LFM_KV_F32) {
+#pragma unroll
+    for (int db = 0; db < 4; ++db) {
+      f32x4 x[2];
+#pragma unroll
+      for (int hb = 0; hb < 2; ++hb)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[hb][i] = __builtin_bit_cast(float, r.v[hb][i][db]);
+      moe::split8(x, op[db]);
+    }
+  } else {
+    u32x4 w[4];
+#pragma unroll
+    for (int hb = 0; hb < 2; ++hb) {
+      const uint32_t(&v)[4][RawTile<FMT>::KW] = r.v[hb];
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {  // keys 4g + 2p and 4g + 2p + 1
+        if constexpr (FMT == LFM_KV_BF16) {
+#pragma unroll
+          for (int db = 0; db < 4; ++db)
+            w[db][2 * hb + p] = __builtin_amdgcn_perm(v[2 * p + 1][db >> 1], v[2 * p][db >> 1],
+                                                      db & 1 ? 0x07060302u : 0x05040100u);
+        } else if constexpr (FMT == LFM_KV_FP8) {
+          // dimensions (0, 1) and (2, 3), the two keys byte by byte
+          const uint32_t q[2] = {__builtin_amdgcn_perm(v[2 * p + 1][0], v[2 * p][0], 0x05010400u),
+                                 __builtin_amdgcn_perm(v[2 * p + 1][0], v[2 * p][0], 0x07030602u)};
+#pragma unroll
+          for (int db = 0; db < 4; ++db)
+            w[db][2 * hb + p] = __builtin_bit_cast(
+                uint32_t, db & 1 ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(q[db >> 1], 1.0f, true)
+                                 : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(q[db >> 1], 1.0f, false));
+        } else {
+#pragma unroll
+          for (int db = 0; db < 4; ++db)
+            w[db][2 * hb + p] = byte_pair((float)(signed char)(v[2 * p][0] >> (8 * db)),
+                                          (float)(signed char)(v[2 * p + 1][0] >> (8 * db)));
+        }
+      }
+    }
+#pragma unroll
+    for (int db = 0; db < 4; ++db) op[db][0] = __builtin_bit_cast(bf16x8, w[db]);
+  }
+}
+
+// One block's part of a product: columns col0 .. of kv head h, every `stride`-th
+// tile of the own positions of sequence b (or, PREFIX, of the shared ones).
+// Tiles are dealt to the parts' waves in turn, so that a wave knows its first
+// tile, and looks up its page, before it knows how long the sequence is.
+template <int FMT, int CT, bool PREFIX, int W>
+__device__ __forceinline__ void flash_part(const KvArgs &a, const FlashArgs &f, int h, int part, int group, int b,
+                                           float *s_lds) {
   using Raw = RawTile<FMT>;
-  constexpr int NP = FMT == LFM_KV_F32 ? 3 : 1;
+  using SH = FlashShape<CT, W>;
+  constexpr int NP = FMT == LFM_KV_F32 ? 3 : 1, NT = SH::NT, COLS = SH::COLS, QP = SH::QP;
+  constexpr bool FEW = SH::FEW;
   // q's parts as operands [column tile][k-step][part][lane], then the waves' sums
-  constexpr bool FEW = CT == 0;
-  constexpr int NT = FEW ? 1 : CT, COLS = FEW ? kFewCols : 16 * CT, QP = FEW ? 1 : 3;
-  constexpr int kSumFloats = kFlashWaves * COLS * kJoinPitch, kPartFloats = NT * 2 * QP * 64 * 4;
-  __shared__ float s_lds[kSumFloats > kPartFloats ? kSumFloats : kPartFloats];
-  __shared__ float2 s_m[kFlashWaves][COLS];
   bf16x8 *const s_q = reinterpret_cast<bf16x8 *>(s_lds);
+  float2 *const s_m = reinterpret_cast<float2 *>(s_lds + SH::kFloats);  // [W][COLS]
   const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  // kv head fastest: with 8 of them a head's keys stay in one XCD's L2
-  const int h = blockIdx.x % a.kv_heads, part = blockIdx.x / a.kv_heads;
-  const int col0 = blockIdx.y * COLS;
   const int lc = FEW ? c & 3 : c;  // the lane's column in its tile
+  const int col0 = group * COLS;
+  const int t0 = part * W + wave;
 
+  const int *table = PREFIX ? a.prefix_pages : a.pages + (size_t)b * a.max_pages;
+  const int most_pages = PREFIX ? (a.prefix_len - 1) >> a.pshift : a.max_pages - 1;
+  int first_pages = 0;  // of the first tile's halves, in lanes 0 and 1
+  if (most_pages >= 0) first_pages = table[min((t0 * kKeys + 16 * (lane & 1)) >> a.pshift, most_pages)];
   KvSeq s;
-  const int *table;
   int len, first_seen;  // keys; those below first_seen are seen by every column of the block
   if (PREFIX) {
     s.row0 = 0;
     s.n = a.tokens;
-    table = a.prefix_pages;
     len = first_seen = a.prefix_len;
   } else {
-    if (!kv_seq<true>(a, blockIdx.z, s)) return;
-    table = a.pages + (size_t)blockIdx.z * a.max_pages;
+    if (!kv_seq<true>(a, b, s)) return;
     len = s.len;
     first_seen = len - s.n + col0 / f.group + 1;
   }
-  if (col0 >= s.n * f.group) return;
-  const int per = part_tiles(len, PREFIX ? f.prefix_parts : f.own_parts);
-  if (part * per * kKeys >= len) return;
-  const bool direct = !PREFIX && f.prefix_parts == 0 && per * kKeys >= len;
+  const int parts = active_parts(len, PREFIX ? f.prefix_parts : f.own_parts), stride = parts * W;
+  if (part >= parts || col0 >= s.n * f.group) return;
+  const bool direct = !PREFIX && f.prefix_parts == 0 && parts == 1;
   // the last position a column of the block sees
   const int seen = PREFIX ? len : min(len, len - s.n + (col0 + COLS - 1) / f.group + 1);
-  const int t_end = min((part + 1) * per, (seen + kKeys - 1) / kKeys);
+  const int t_end = (seen + kKeys - 1) / kKeys;
 
-  // Pages of the wave's next 32 tiles, a half tile's in each lane (-1 outside the cache).
-  const int t0 = part * per + wave;
-  int pages = 0;
-  auto find_pages = [&](int t) {
-    const int k0 = min((t + kFlashWaves * (lane >> 1)) * kKeys + 16 * (lane & 1), (len - 1) & ~15);
-    pages = table[k0 >> a.pshift];
-    if (pages < 0 || pages >= a.num_pages) {
-      kv_flag(a.bad);
-      pages = -1;
-    }
-  };
-  find_pages(t0);
-
-  // q's parts, scaled so that a score is the log2 of its weight; wave w prepares
-  // the column tiles' k-steps w, w + 4, ...
+  // q, for the column tiles' k-steps w, w + W, ... in wave w
+  constexpr int QE = (2 * NT + W - 1) / W;
+  f32x4 qv[QE][2];
   int last[NT];  // last position the lane's columns see
 #pragma unroll
   for (int ct = 0; ct < NT; ++ct) last[ct] = PREFIX ? len - 1 : len - s.n + (col0 + ct * 16 + lc) / f.group;
-  for (int e = wave; e < 2 * NT; e += kFlashWaves) {
-    const int ct = e >> 1, st = e & 1;
-    const int col = col0 + ct * 16 + lc, tok = col / f.group, qh = h * f.group + col - tok * f.group;
+#pragma unroll
+  for (int n = 0; n < QE; ++n) {
+    const int e = min(wave + n * W, 2 * NT - 1), col = col0 + (e >> 1) * 16 + lc, tok = col / f.group;
     const bool valid = tok < s.n;
-    const float *qr = f.q + (size_t)(s.row0 + (valid ? tok : 0)) * f.ld + qh * kRowDim;
-    float x[8];
+    const float *qr = f.q + (size_t)(s.row0 + (valid ? tok : 0)) * f.ld + (h * f.group + col - tok * f.group) * kRowDim;
 #pragma unroll
-    for (int j = 0; j < 8; j += 4) {
-      const f32x4 v = moe::ld4(qr + key_dim<FMT>(st, g, j));
-#pragma unroll
-      for (int i = 0; i < 4; ++i) x[j + i] = valid ? v[i] * (0.125f * 1.44269504088896340736f) : 0.0f;
-    }
-    if constexpr (FEW) {
-      s_q[e * 64 + lane] = part8(x, c >> 2);
-    } else {
-      bf16x8 part3[3];
-      split8_exact(x, part3);
-#pragma unroll
-      for (int q = 0; q < 3; ++q) s_q[(e * 3 + q) * 64 + lane] = part3[q];
+    for (int j = 0; j < 2; ++j) {
+      qv[n][j] = moe::ld4(qr + key_dim<FMT>(e & 1, g, 4 * j));
+      if (!valid) qv[n][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
   }
 
-  f32x4 o[NT][4];
-  float m[NT], l[NT];
-#pragma unroll
-  for (int ct = 0; ct < NT; ++ct) {
-    m[ct] = kNoScore;
-    l[ct] = 0.0f;
-#pragma unroll
-    for (int d = 0; d < 4; ++d) o[ct][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  }
-
-  auto load = [&](int n, Raw &r) {  // the wave's n-th tile
-    const int t = t0 + n * kFlashWaves;
-    if (n > 0 && (n & 31) == 0) find_pages(t);
+  auto in_cache = [&](int page) {
+    if (page >= 0 && page < a.num_pages) return page;
+    kv_flag(a.bad);
+    return -1;
+  };
+  auto load = [&](int t, int page0, int page1, Raw &r) {
 #pragma unroll
     for (int hb = 0; hb < 2; ++hb) {
-      const int k0 = min(t * kKeys + 16 * hb, (len - 1) & ~15);
-      const int page = __builtin_amdgcn_readlane(pages, 2 * (n & 31) + hb);
+      // a half tile behind the last key repeats the one with that key
+      const int k0 = min(t * kKeys + 16 * hb, (len - 1) & ~15), page = hb ? page1 : page0;
       r.ok[hb] = page >= 0;
       const size_t row = kv_row(a, max(page, 0), h, k0 & ((1 << a.pshift) - 1));
       const char *kp = a.k + row * kRowDim * kv_size<FMT>(), *vp = a.v + row * kRowDim * kv_size<FMT>();
@@ -382,110 +439,78 @@ void kv_flash_kernel(KvArgs a, FlashArgs f) {
       }
     }
   };
+  // Pages of 32 of the wave's tiles, a half tile's in each lane (-1 outside the cache).
+  auto page_of = [&](int t) {
+    return table[min((t + stride * (lane >> 1)) * kKeys + 16 * (lane & 1), (len - 1) & ~15) >> a.pshift];
+  };
 
-  auto compute = [&](int t, Raw &r) {
+  f32x4 o[NT][4];
+  // ref: the running maximum, 0 before there is one; limit: what a score may pass it by
+  float ref[NT], limit[NT], l[NT];
+#pragma unroll
+  for (int ct = 0; ct < NT; ++ct) {
+    ref[ct] = l[ct] = 0.0f;
+    limit[ct] = kNoScore;
+#pragma unroll
+    for (int d = 0; d < 4; ++d) o[ct][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+
+  // Tile t from r, which then takes tile `next`, on pages next0 and next1.
+  auto tile = [&](int t, Raw &r, int next, int next0, int next1) {
     const int k0 = t * kKeys;
-    const bool cut = k0 + kKeys > first_seen || !r.ok[0] || !r.ok[1];  // wave-uniform
-    // operands of K
-    bf16x8 kop[2][2][NP];
-#pragma unroll
-    for (int hb = 0; hb < 2; ++hb)
-#pragma unroll
-      for (int st = 0; st < 2; ++st) {
-        if constexpr (FMT == LFM_KV_F32) {
-          const f32x4 x[2] = {__builtin_bit_cast(f32x4, r.k[hb][2 * st]), __builtin_bit_cast(f32x4, r.k[hb][2 * st + 1])};
-          moe::split8(x, kop[hb][st]);
-        } else if constexpr (FMT == LFM_KV_BF16) {
-          kop[hb][st][0] = __builtin_bit_cast(bf16x8, r.k[hb][st]);
-        } else {
-          u32x4 w;
-          uint32_t lo, hi;
-          widen4<FMT>(r.k[hb][0][2 * st], lo, hi);
-          w[0] = lo;
-          w[1] = hi;
-          widen4<FMT>(r.k[hb][0][2 * st + 1], lo, hi);
-          w[2] = lo;
-          w[3] = hi;
-          kop[hb][st][0] = __builtin_bit_cast(bf16x8, w);
-        }
-      }
-    // values of keys behind the sequence's end or on no page: zero
-    if (cut) {
-#pragma unroll
-      for (int hb = 0; hb < 2; ++hb)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const bool there = r.ok[hb] && k0 + 16 * hb + 4 * g + i < len;
-#pragma unroll
-          for (int w = 0; w < Raw::KW; ++w) r.v[hb][i][w] = there ? r.v[hb][i][w] : 0u;
-        }
-    }
-    // operands of V: block db takes dimension 4c + db of the lane's eight keys
-    bf16x8 vop[4][NP];
-    if constexpr (FMT == LFM_KV_F32) {
-#pragma unroll
-      for (int db = 0; db < 4; ++db) {
-        f32x4 x[2];
-#pragma unroll
-        for (int hb = 0; hb < 2; ++hb)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) x[hb][i] = __builtin_bit_cast(float, r.v[hb][i][db]);
-        moe::split8(x, vop[db]);
-      }
-    } else {
-      u32x4 w[4];
-#pragma unroll
-      for (int hb = 0; hb < 2; ++hb) {
-        const uint32_t(&v)[4][Raw::KW] = r.v[hb];
-        if constexpr (FMT == LFM_KV_BF16) {
-#pragma unroll
-          for (int p = 0; p < 2; ++p)
-#pragma unroll
-            for (int db = 0; db < 4; ++db)
-              w[db][2 * hb + p] = __builtin_amdgcn_perm(v[2 * p + 1][db >> 1], v[2 * p][db >> 1],
-                                                        db & 1 ? 0x07060302u : 0x05040100u);
-        } else if constexpr (FMT == LFM_KV_FP8) {
-          uint32_t q[2][2];  // keys 2p and 2p+1, dimensions (0, 1) and (2, 3), byte by byte
-#pragma unroll
-          for (int p = 0; p < 2; ++p) {
-            q[p][0] = __builtin_amdgcn_perm(v[2 * p + 1][0], v[2 * p][0], 0x05010400u);
-            q[p][1] = __builtin_amdgcn_perm(v[2 * p + 1][0], v[2 * p][0], 0x07030602u);
-          }
-#pragma unroll
-          for (int p = 0; p < 2; ++p)
-#pragma unroll
-            for (int db = 0; db < 4; ++db)
-              w[db][2 * hb + p] = __builtin_bit_cast(
-                  uint32_t, db & 1 ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(q[p][db >> 1], 1.0f, true)
-                                   : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(q[p][db >> 1], 1.0f, false));
-        } else {
-#pragma unroll
-          for (int p = 0; p < 2; ++p)
-#pragma unroll
-            for (int db = 0; db < 4; ++db)
-              w[db][2 * hb + p] = byte_pair((float)(signed char)(v[2 * p][0] >> (8 * db)),
-                                            (float)(signed char)(v[2 * p + 1][0] >> (8 * db)));
-        }
-      }
-#pragma unroll
-      for (int db = 0; db < 4; ++db) vop[db][0] = __builtin_bit_cast(bf16x8, w[db]);
-    }
+    const bool ok[2] = {r.ok[0], r.ok[1]};
+    // some keys are behind the end, behind a column's own position or on no page (wave-uniform)
+    const bool cut = k0 + kKeys > first_seen || !ok[0] || !ok[1];
+    f32x4 ks[2], vs[2];
+    bf16x8 kop[2][2][NP], vop[4][NP];
     // A value that is not finite must not meet the zero weight of a column that
     // does not see it: such values (a bit each in nf) leave the product and make
     // the outputs of the columns that do see them NaN.
     uint32_t nf = 0;
+    if constexpr (Raw::SCALED) {
+#pragma unroll
+      for (int hb = 0; hb < 2; ++hb) {
+        ks[hb] = r.ks[hb];
+        vs[hb] = r.vs[hb];
+      }
+    }
+    if (cut) {  // values of keys behind the sequence's end or on no page: zero
+#pragma unroll
+      for (int hb = 0; hb < 2; ++hb)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const bool there = ok[hb] && k0 + 16 * hb + 4 * g + i < len;
+#pragma unroll
+          for (int w = 0; w < Raw::KW; ++w) r.v[hb][i][w] = there ? r.v[hb][i][w] : 0u;
+          if constexpr (Raw::SCALED) {
+            const float x = vs[hb][i];
+            const bool finite = PREFIX || __builtin_fabsf(x) <= __FLT_MAX__;  // all see the prefix
+            if (there && !finite) nf |= 0x01010101u << (4 * hb + i);
+            vs[hb][i] = there && finite ? x : 0.0f;
+          }
+        }
+    }
+#pragma unroll
+    for (int hb = 0; hb < 2; ++hb)
+#pragma unroll
+      for (int st = 0; st < 2; ++st) key_operand<FMT>(r, hb, st, kop[hb][st]);
+    value_operands<FMT>(r, vop);
+    load(next, next0, next1, r);
+
     bool apart = false;
-    if (FMT != LFM_KV_INT8 && !PREFIX && cut) {
+    if (!PREFIX && cut) {
+      if constexpr (FMT != LFM_KV_INT8) {
 #pragma unroll
-      for (int db = 0; db < 4; ++db) {
-        const u32x4 w = __builtin_bit_cast(u32x4, vop[db][0]);
+        for (int db = 0; db < 4; ++db) {
+          const u32x4 w = __builtin_bit_cast(u32x4, vop[db][0]);
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          nf |= ((w[j] & 0x7F80u) == 0x7F80u ? 1u : 0u) << (8 * db + 2 * j) |
-                ((w[j] & 0x7F800000u) == 0x7F800000u ? 2u : 0u) << (8 * db + 2 * j);
+          for (int j = 0; j < 4; ++j)
+            nf |= ((w[j] & 0x7F80u) == 0x7F80u ? 1u : 0u) << (8 * db + 2 * j) |
+                  ((w[j] & 0x7F800000u) == 0x7F800000u ? 2u : 0u) << (8 * db + 2 * j);
+        }
       }
       apart = __any(nf != 0);
-      if (apart) {
+      if (apart && FMT != LFM_KV_INT8) {
 #pragma unroll
         for (int db = 0; db < 4; ++db)
 #pragma unroll
@@ -498,9 +523,10 @@ void kv_flash_kernel(KvArgs a, FlashArgs f) {
       }
     }
 
+    // scores of keys 16 hb + 4g + i against the running maximum
+    float p[NT][8];
 #pragma unroll
     for (int ct = 0; ct < NT; ++ct) {
-      float p[8];  // scores, then weights, of keys 16 hb + 4g + i
       bf16x8 qp[2][QP];
 #pragma unroll
       for (int e = 0; e < 2 * QP; ++e) qp[e / QP][e % QP] = s_q[(ct * 2 * QP + e) * 64 + lane];
@@ -509,55 +535,75 @@ void kv_flash_kernel(KvArgs a, FlashArgs f) {
         f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int st = 0; st < 2; ++st) acc = mfma_parts(kop[hb][st], qp[st], acc);
-        if constexpr (FEW) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) acc[i] = sum_parts(acc[i]);
+        for (int i = 0; i < 4; ++i) {
+          const float sc = FEW ? sum_parts(acc[i]) : (float)acc[i];
+          p[ct][4 * hb + i] = Raw::SCALED ? __builtin_fmaf(sc, ks[hb][i], -ref[ct]) : sc - ref[ct];
         }
-        if constexpr (Raw::SCALED) acc *= r.ks[hb];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) p[4 * hb + i] = acc[i];
       }
-      if (cut) {
+    }
+    if (cut) {
+#pragma unroll
+      for (int ct = 0; ct < NT; ++ct)
 #pragma unroll
         for (int e = 0; e < 8; ++e)
-          if (!r.ok[e >> 2] || k0 + 16 * (e >> 2) + 4 * g + (e & 3) > last[ct]) p[e] = kNoScore;
-      }
-      float mt = p[0];
+          p[ct][e] = !ok[e >> 2] || k0 + 16 * (e >> 2) + 4 * g + (e & 3) > last[ct] ? kNoScore : p[ct][e];
+    }
+    bool raise = false;
 #pragma unroll
-      for (int e = 1; e < 8; ++e) mt = fmaxf(mt, p[e]);
-      if (__any(mt > m[ct] + kRaise)) {
+    for (int ct = 0; ct < NT; ++ct) {
+      float top = __builtin_elementwise_maximum(p[ct][0], p[ct][1]);
+#pragma unroll
+      for (int e = 2; e < 8; e += 2)
+        top = __builtin_elementwise_maximum(__builtin_elementwise_maximum(p[ct][e], p[ct][e + 1]), top);
+      raise = raise || top > limit[ct];
+    }
+    if (__any(raise)) {
+#pragma unroll
+      for (int ct = 0; ct < NT; ++ct) {
+        float mt = kNoScore;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) mt = fmaxf(mt, p[ct][e]);
         mt = fmaxf(mt, __shfl_xor(mt, 16));
         mt = fmaxf(mt, __shfl_xor(mt, 32));
-        const float mn = fmaxf(m[ct], mt);
-        const float scale = mn == kNoScore ? 1.0f : __builtin_amdgcn_exp2f(m[ct] - mn);
-        m[ct] = mn;
-        l[ct] *= scale;
+        const bool had = limit[ct] != kNoScore;
+        if (had) mt = fmaxf(mt, 0.0f);
+        if (mt != kNoScore) {
+          const float to = ref[ct] + mt, by = to - ref[ct];  // what the rounded maximum is above the old one
+          const float scale = had ? __builtin_amdgcn_exp2f(-by) : 0.0f;
+          ref[ct] = to;
+          limit[ct] = kRaise;
+          l[ct] *= scale;
 #pragma unroll
-        for (int d = 0; d < 4; ++d) o[ct][d] *= scale;
+          for (int d = 0; d < 4; ++d) o[ct][d] *= scale;
+          // of scores beyond 2^27 the FMA keeps more than their maximum's rounding left
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            p[ct][e] -= by;
+            p[ct][e] = p[ct][e] > kRaise ? kRaise : p[ct][e];
+          }
+        }
       }
-      const float ref = m[ct] == kNoScore ? 0.0f : m[ct];
+    }
+#pragma unroll
+    for (int ct = 0; ct < NT; ++ct) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        p[e] = __builtin_amdgcn_exp2f(p[e] - ref);
-        l[ct] += p[e];
-      }
-      if constexpr (Raw::SCALED) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) p[e] *= r.vs[e >> 2][e & 3];
-        if (cut) {  // a scale there may be anything
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (!r.ok[e >> 2] || k0 + 16 * (e >> 2) + 4 * g + (e & 3) > last[ct]) p[e] = 0.0f;
-        }
+        p[ct][e] = __builtin_amdgcn_exp2f(p[ct][e]);
+        l[ct] += p[ct][e];
+        if constexpr (Raw::SCALED) p[ct][e] *= vs[e >> 2][e & 3];
       }
       bf16x8 pp[QP];
       if constexpr (FEW)
-        pp[0] = part8(p, c >> 2);
+        pp[0] = part8(p[ct], c >> 2);
       else
-        split8_exact(p, pp);
+        split8_exact(p[ct], pp);
 #pragma unroll
       for (int d = 0; d < 4; ++d) o[ct][d] = mfma_parts(vop[d], pp, o[ct][d]);
-      if (apart) {
+    }
+    if (apart) {
+#pragma unroll
+      for (int ct = 0; ct < NT; ++ct) {
         // how many of them a column sees: a product of ones
         u32x4 see;
 #pragma unroll
@@ -580,15 +626,39 @@ void kv_flash_kernel(KvArgs a, FlashArgs f) {
     }
   };
 
-  // Two tiles in registers: one computed, one on its way.  The load past the
-  // wave's last tile repeats that one (its lines are in L2).
-  Raw ra, rb;
-  if (t0 < t_end) load(0, ra);
+  Raw r;
+  int pages = 0;
+  if (t0 < t_end) {
+    pages = in_cache(page_of(t0));
+    const int half0 = __builtin_amdgcn_readlane(first_pages, 0);
+    const int half1 = t0 * kKeys + 16 < len ? __builtin_amdgcn_readlane(first_pages, 1) : half0;
+    load(t0, in_cache(half0), in_cache(half1), r);
+  }
+  // q's parts, scaled so that a score is the log2 of its weight
+#pragma unroll
+  for (int n = 0; n < QE; ++n) {
+    const int e = min(wave + n * W, 2 * NT - 1);  // a surplus wave repeats the last
+    float x[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) x[j] = qv[n][j >> 2][j & 3] * (0.125f * 1.44269504088896340736f);
+    if constexpr (FEW) {
+      s_q[e * 64 + lane] = part8(x, c >> 2);
+    } else {
+      bf16x8 part3[3];
+      split8_exact(x, part3);
+#pragma unroll
+      for (int q = 0; q < 3; ++q) s_q[(e * 3 + q) * 64 + lane] = part3[q];
+    }
+  }
   __syncthreads();  // q's parts are there
-  for (int t = t0, n = 0; t < t_end; t += kFlashWaves, ++n) {
-    load(t + kFlashWaves < t_end ? n + 1 : n, rb);
-    compute(t, ra);
-    ra = rb;
+  for (int t = t0, n = 0; t < t_end; t += stride, ++n) {
+    // the next tile's loads set out once this one's are operands; behind the
+    // wave's last tile that one is loaded again (its lines are in L2)
+    const bool more = t + stride < t_end;
+    const int i = (n + (more ? 1 : 0)) & 31;
+    if (more && i == 0) pages = in_cache(page_of(t + stride));
+    tile(t, r, more ? t + stride : t, __builtin_amdgcn_readlane(pages, 2 * i),
+         __builtin_amdgcn_readlane(pages, 2 * i + 1));
   }
   __syncthreads();  // and read for the last time
 
@@ -605,7 +675,7 @@ void kv_flash_kernel(KvArgs a, FlashArgs f) {
         for (int i = 0; i < 4; ++i) o[ct][d][i] = sum_parts(o[ct][d][i]);
     }
     if (c < COLS) {
-      if (g == 0) s_m[wave][ct * 16 + c] = float2{m[ct], l[ct]};
+      if (g == 0) s_m[wave * COLS + ct * 16 + c] = float2{limit[ct] == kNoScore ? kNoScore : ref[ct], l[ct]};
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         moe::st4(&s_lds[(wave * COLS + ct * 16 + c) * kJoinPitch + 16 * g + 4 * i],
@@ -614,21 +684,19 @@ void kv_flash_kernel(KvArgs a, FlashArgs f) {
   }
   __syncthreads();
 #pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    const int e = n * kFlashThreads + threadIdx.x, cc = e >> 4, d = (e & 15) * 4;
+  for (int n = 0; n < (COLS * 16 + 64 * W - 1) / (64 * W); ++n) {
+    const int e = n * 64 * W + threadIdx.x, cc = e >> 4, d = (e & 15) * 4;
     const int col = col0 + cc, tok = col / f.group, qh = h * f.group + col - tok * f.group;
     if (cc >= COLS || tok >= s.n) continue;
-    float mw[kFlashWaves], mx = kNoScore, lt = 0.0f;
+    float mx = kNoScore, lt = 0.0f;
 #pragma unroll
-    for (int w = 0; w < kFlashWaves; ++w) {
-      mw[w] = s_m[w][cc].x;
-      mx = fmaxf(mx, mw[w]);
-    }
+    for (int w = 0; w < W; ++w) mx = fmaxf(mx, s_m[w * COLS + cc].x);
     f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int w = 0; w < kFlashWaves; ++w) {
-      const float sc = part_scale(float2{mw[w], s_m[w][cc].y}, mx);
-      lt += s_m[w][cc].y * sc;
+    for (int w = 0; w < W; ++w) {
+      const float2 ml = s_m[w * COLS + cc];
+      const float sc = part_scale(ml, mx);
+      lt += ml.y * sc;
       v += moe::ld4(&s_lds[(w * COLS + cc) * kJoinPitch + d]) * sc;
     }
     const size_t row = (size_t)(s.row0 + tok) * f.heads + qh;
@@ -643,6 +711,18 @@ void kv_flash_kernel(KvArgs a, FlashArgs f) {
   }
 }
 
+// Waves a SIMD holds, by the registers a tile's columns take.
+constexpr int flash_waves(int fmt, int ct) { return fmt == LFM_KV_F32 ? 2 : ct == 0 ? 4 : ct == 1 ? 3 : 2; }
+
+// kv head fastest: with 8 of them a head's keys stay in one XCD's L2.
+template <int FMT, int CT, bool PREFIX>
+__global__ __launch_bounds__(64 * column_waves(CT)) __attribute__((amdgpu_waves_per_eu(flash_waves(FMT, CT))))
+void kv_flash_kernel(KvArgs a, FlashArgs f) {
+  constexpr int W = column_waves(CT);
+  __shared__ float s_lds[FlashShape<CT, W>::kBytes / 4];
+  flash_part<FMT, CT, PREFIX, W>(a, f, blockIdx.x % a.kv_heads, blockIdx.x / a.kv_heads, blockIdx.y, blockIdx.z, s_lds);
+}
+
 // Joins the parts of a token's head, a wave per row: 16 lanes take a part's 64
 // sums, so four parts are loaded at a time, and a lane a part's maximum.
 __global__ __launch_bounds__(256) void kv_join_kernel(KvArgs a, FlashArgs f) {
@@ -650,14 +730,12 @@ __global__ __launch_bounds__(256) void kv_join_kernel(KvArgs a, FlashArgs f) {
   if (!kv_seq<true>(a, blockIdx.y, s)) return;
   const int r = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
   if (r >= s.n * f.heads) return;
-  const int own_per = part_tiles(s.len, f.own_parts) * kKeys, own = (s.len + own_per - 1) / own_per;
+  const int own = active_parts(s.len, f.own_parts);
   int parts = own;
-  if (f.prefix_parts > 0) {
-    const int per = part_tiles(a.prefix_len, f.prefix_parts) * kKeys;
-    parts += (a.prefix_len + per - 1) / per;
-  } else if (own == 1) {
+  if (f.prefix_parts > 0)
+    parts += active_parts(a.prefix_len, f.prefix_parts);
+  else if (own == 1)
     return;  // written by its one block
-  }
   const size_t row = (size_t)s.row0 * f.heads + r;
   const int tok = r / f.heads, qh = r - tok * f.heads;
   auto at = [&](int p) { return (size_t)(p < own ? p : f.own_parts + p - own) * f.rows + row; };
@@ -749,9 +827,8 @@ static int column_tiles(long long cols) { return cols <= kFewCols ? 0 : cols <= 
 static int columns_of(int ct) { return ct == 0 ? kFewCols : 16 * ct; }
 
 static int parts_of(long long keys, long long blocks, int ct) {
-  const long long tiles = (keys + kKeys - 1) / kKeys, most = std::max<long long>(1, tiles / kMinTiles);
-  const long long want = ct <= 1 ? kFlashBlocks : kWideBlocks;
-  return (int)std::min<long long>({most, std::max<long long>(1, (want + blocks - 1) / blocks), 256});
+  const long long want = ct == 1 ? kFlashBlocks : kWideBlocks;
+  return active_parts((int)keys, (int)std::min<long long>(std::max<long long>(1, (want + blocks - 1) / blocks), 256));
 }
 
 static FlashPlan flash_plan(const KvArgs &a, int heads) {
@@ -781,12 +858,12 @@ size_t kv_attention_ws(const KvArgs &a, int heads) {
 template <int FMT, bool PREFIX>
 static hipError_t kv_flash_launch(const KvArgs &a, const FlashArgs &f, int ct, dim3 grid, hipStream_t st) {
   switch (ct) {
-    case 0: hipLaunchKernelGGL((kv_flash_kernel<FMT, 0, PREFIX>), grid, dim3(kFlashThreads), 0, st, a, f); break;
-    case 1: hipLaunchKernelGGL((kv_flash_kernel<FMT, 1, PREFIX>), grid, dim3(kFlashThreads), 0, st, a, f); break;
-    case 2: hipLaunchKernelGGL((kv_flash_kernel<FMT, 2, PREFIX>), grid, dim3(kFlashThreads), 0, st, a, f); break;
+    case 0: hipLaunchKernelGGL((kv_flash_kernel<FMT, 0, PREFIX>), grid, dim3(64 * column_waves(0)), 0, st, a, f); break;
+    case 1: hipLaunchKernelGGL((kv_flash_kernel<FMT, 1, PREFIX>), grid, dim3(64 * column_waves(1)), 0, st, a, f); break;
+    case 2: hipLaunchKernelGGL((kv_flash_kernel<FMT, 2, PREFIX>), grid, dim3(64 * column_waves(2)), 0, st, a, f); break;
     default:
       if constexpr (FMT != LFM_KV_F32)
-        hipLaunchKernelGGL((kv_flash_kernel<FMT, 4, PREFIX>), grid, dim3(kFlashThreads), 0, st, a, f);
+        hipLaunchKernelGGL((kv_flash_kernel<FMT, 4, PREFIX>), grid, dim3(64 * column_waves(4)), 0, st, a, f);
   }
   return hipGetLastError();
 }

@@ -353,6 +353,38 @@ def test_attention_does_not_see_the_future(fmt):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("at", [3, 39])
+def test_not_finite_rows_reach_who_sees_them(fmt, at):
+    """A row of the prefix reaches every token; one of a kv head's keys or values only its heads."""
+    r = np.random.default_rng(fmt)
+    pool = Pool(fmt, 8, 16, 40)
+    q = Seqs(r, pool, [4, 1], [50, 35], prefix=40)
+    fill(r, pool, q)
+    x = draws(r, (q.tokens, 2048), sizes=False)
+    clean = attend(pool, q, x, 32)
+    for which in range(2):
+        for val in (np.nan, np.inf):
+            rows = [np.ones((1, 8, 64), np.float32) for _ in range(2)]
+            rows[which][:, 3] = val
+            saved = [a.copy() for a in pool.data + pool.scale]
+            pg, off = q.front[at // 16], at % 16
+            for i in range(2):
+                d, sc = R.store(rows[i], fmt)
+                pool.data[i][pg, 3, off] = d[0, 3]
+                if sc is not None:
+                    pool.scale[i][pg, 3, off] = sc[0, 3]
+            pool.upload()
+            got = attend(pool, q, x, 32).reshape(-1, 32, 64)
+            assert not np.isfinite(got[:, 12:16]).any()
+            keep = np.r_[0:12, 16:32]
+            assert np.array_equal(bits(got[:, keep]), bits(clean.reshape(-1, 32, 64)[:, keep]))
+            for a, b in zip(pool.data + pool.scale, saved):
+                a[...] = b
+            pool.upload()
+
+
+@pytest.mark.gpu
 def test_attention_of_not_finite_queries():
     r = np.random.default_rng(1)
     pool = Pool(R.INT8, 8, 16, 40)
