@@ -151,8 +151,8 @@ __host__ __device__ inline int active_parts(int keys, int parts) {
   return most < 1 ? 1 : most < parts ? most : parts;
 }
 
-// Waves of a block: one token's few columns leave room, and time, for eight.
-__host__ __device__ constexpr int column_waves(int ct) { return ct == 0 ? 8 : 4; }
+// Waves of a block without a prefix beside it: few columns leave room for eight.
+__host__ __device__ constexpr int own_waves(int ct) { return ct == 0 ? 8 : 4; }
 
 // A block of W waves with CT tiles of 16 columns; CT = 0: kFewCols columns, whose
 // three parts fill a tile.
@@ -714,13 +714,37 @@ __device__ __forceinline__ void flash_part(const KvArgs &a, const FlashArgs &f, 
 // Waves a SIMD holds, by the registers a tile's columns take.
 constexpr int flash_waves(int fmt, int ct) { return fmt == LFM_KV_F32 ? 2 : ct == 0 ? 4 : ct == 1 ? 3 : 2; }
 
-// kv head fastest: with 8 of them a head's keys stay in one XCD's L2.
-template <int FMT, int CT, bool PREFIX>
-__global__ __launch_bounds__(64 * column_waves(CT)) __attribute__((amdgpu_waves_per_eu(flash_waves(FMT, CT))))
+// Own positions alone.  kv head fastest: with 8 of them a head's keys stay in one
+// XCD's L2.
+template <int FMT, int CT>
+__global__ __launch_bounds__(64 * own_waves(CT)) __attribute__((amdgpu_waves_per_eu(flash_waves(FMT, CT))))
 void kv_flash_kernel(KvArgs a, FlashArgs f) {
-  constexpr int W = column_waves(CT);
-  __shared__ float s_lds[FlashShape<CT, W>::kBytes / 4];
-  flash_part<FMT, CT, PREFIX, W>(a, f, blockIdx.x % a.kv_heads, blockIdx.x / a.kv_heads, blockIdx.y, blockIdx.z, s_lds);
+  __shared__ float s_lds[FlashShape<CT, own_waves(CT)>::kBytes / 4];
+  flash_part<FMT, CT, false, own_waves(CT)>(a, f, blockIdx.x % a.kv_heads, blockIdx.x / a.kv_heads, blockIdx.y,
+                                            blockIdx.z, s_lds);
+}
+
+// The prefix, whose blocks are the grid's first, and the own positions beside it.
+template <int FMT, int PCT, int CT>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(flash_waves(FMT, PCT))))
+void kv_prefix_flash_kernel(KvArgs a, FlashArgs f, int prefix_blocks, int own_groups) {
+  constexpr int W = 4;
+  using P = FlashShape<PCT, W>;
+  using O = FlashShape<CT, W>;
+  __shared__ float s_lds[(P::kBytes > O::kBytes ? P::kBytes : O::kBytes) / 4];
+  int at = blockIdx.x;
+  if (at < prefix_blocks) {
+    const int h = at % a.kv_heads;
+    at /= a.kv_heads;
+    flash_part<FMT, PCT, true, W>(a, f, h, at % f.prefix_parts, at / f.prefix_parts, 0, s_lds);
+  } else {
+    at -= prefix_blocks;
+    const int h = at % a.kv_heads;
+    at /= a.kv_heads;
+    const int part = at % f.own_parts;
+    at /= f.own_parts;
+    flash_part<FMT, CT, false, W>(a, f, h, part, at % own_groups, at / own_groups, s_lds);
+  }
 }
 
 // Joins the parts of a token's head, a wave per row: 16 lanes take a part's 64
@@ -815,34 +839,34 @@ hipError_t launch_kv_read(const KvArgs &a, float *k_out, float *v_out, int rows,
 }
 
 // How a call is split: column tiles a wave holds, and parts of the own positions
-// and of the prefix so that about kFlashBlocks blocks run.
-constexpr int kFlashBlocks = 1024, kWideBlocks = 512;
+// and of the prefix so that about as many blocks run as the CUs hold.
+constexpr int kOwnBlocks = 512, kOneTileBlocks = 1024, kPrefixBlocks = 256;
 
 struct FlashPlan {
   int own_ct, prefix_ct, own_groups, prefix_groups, own_parts, prefix_parts;
 };
 
-static int column_tiles(long long cols) { return cols <= kFewCols ? 0 : cols <= 16 ? 1 : cols <= 32 ? 2 : 4; }
-
 static int columns_of(int ct) { return ct == 0 ? kFewCols : 16 * ct; }
 
-static int parts_of(long long keys, long long blocks, int ct) {
-  const long long want = ct == 1 ? kFlashBlocks : kWideBlocks;
+static int widest(int format) { return format == LFM_KV_F32 ? 2 : 4; }
+
+static int parts_of(long long keys, long long blocks, long long want) {
   return active_parts((int)keys, (int)std::min<long long>(std::max<long long>(1, (want + blocks - 1) / blocks), 256));
 }
 
 static FlashPlan flash_plan(const KvArgs &a, int heads) {
   FlashPlan p{};
   const long long group = heads / a.kv_heads, cap = (long long)a.max_pages << a.pshift;
-  const int widest = a.format == LFM_KV_F32 ? 2 : 4;
-  p.own_ct = std::min(widest, column_tiles(a.max_new * group));
-  p.own_groups = (int)((a.max_new * group + columns_of(p.own_ct) - 1) / columns_of(p.own_ct));
+  const long long own = a.max_new * group, all = a.tokens * group;
+  p.own_ct = own <= kFewCols ? 0 : own <= 16 ? 1 : std::min(widest(a.format), own <= 32 ? 2 : 4);
+  p.own_groups = (int)((own + columns_of(p.own_ct) - 1) / columns_of(p.own_ct));
   p.own_parts = parts_of(std::min<long long>(a.max_len ? a.max_len : cap, cap),
-                         (long long)p.own_groups * a.kv_heads * std::max(a.batch, 1), p.own_ct);
+                         (long long)p.own_groups * a.kv_heads * std::max(a.batch, 1),
+                         p.own_ct == 1 ? kOneTileBlocks : kOwnBlocks);
   if (a.prefix_len > 0) {
-    p.prefix_ct = std::min(widest, column_tiles(a.tokens * group));
-    p.prefix_groups = (int)((a.tokens * group + columns_of(p.prefix_ct) - 1) / columns_of(p.prefix_ct));
-    p.prefix_parts = parts_of(a.prefix_len, (long long)p.prefix_groups * a.kv_heads, p.prefix_ct);
+    p.prefix_ct = all <= 16 && p.own_ct <= 1 ? 1 : widest(a.format);
+    p.prefix_groups = (int)((all + columns_of(p.prefix_ct) - 1) / columns_of(p.prefix_ct));
+    p.prefix_parts = parts_of(a.prefix_len, (long long)p.prefix_groups * a.kv_heads, kPrefixBlocks);
   }
   return p;
 }
@@ -855,17 +879,15 @@ size_t kv_attention_ws(const KvArgs &a, int heads) {
   return parts == 1 ? 0 : flash_rows(a, heads) * parts * (kRowDim + 2) * sizeof(float);
 }
 
-template <int FMT, bool PREFIX>
-static hipError_t kv_flash_launch(const KvArgs &a, const FlashArgs &f, int ct, dim3 grid, hipStream_t st) {
+// f with `ct` as a compile-time constant.
+template <int MOST, typename F>
+static hipError_t by_columns(int ct, F &&f) {
   switch (ct) {
-    case 0: hipLaunchKernelGGL((kv_flash_kernel<FMT, 0, PREFIX>), grid, dim3(64 * column_waves(0)), 0, st, a, f); break;
-    case 1: hipLaunchKernelGGL((kv_flash_kernel<FMT, 1, PREFIX>), grid, dim3(64 * column_waves(1)), 0, st, a, f); break;
-    case 2: hipLaunchKernelGGL((kv_flash_kernel<FMT, 2, PREFIX>), grid, dim3(64 * column_waves(2)), 0, st, a, f); break;
-    default:
-      if constexpr (FMT != LFM_KV_F32)
-        hipLaunchKernelGGL((kv_flash_kernel<FMT, 4, PREFIX>), grid, dim3(64 * column_waves(4)), 0, st, a, f);
+    case 0: return f(std::integral_constant<int, 0>{});
+    case 1: return f(std::integral_constant<int, 1>{});
+    case 2: return f(std::integral_constant<int, 2>{});
+    default: return f(std::integral_constant<int, MOST>{});
   }
-  return hipGetLastError();
 }
 
 hipError_t launch_kv_attention(const KvArgs &a, const float *q, int ld, float *out, int ldo, int heads, void *ws,
@@ -875,13 +897,24 @@ hipError_t launch_kv_attention(const KvArgs &a, const float *q, int ld, float *o
   float *po = static_cast<float *>(ws);
   const FlashArgs f{q, out, po, reinterpret_cast<float2 *>(po + rows * (p.own_parts + p.prefix_parts) * kRowDim),
                     ld, ldo, heads, heads / a.kv_heads, p.own_parts, p.prefix_parts, rows};
-  if (p.own_groups > 65535 || p.prefix_groups > 65535) return hipErrorInvalidValue;
+  const long long own_blocks = (long long)a.kv_heads * p.own_parts * p.own_groups * a.batch;
+  const long long prefix_blocks = (long long)a.kv_heads * p.prefix_parts * p.prefix_groups;
+  if (p.own_groups > 65535 || own_blocks + prefix_blocks > 0x7FFFFFFF) return hipErrorInvalidValue;
   return by_format(a.format, [&](auto fmt) -> hipError_t {
-    hipError_t e = hipSuccess;
-    if (p.prefix_parts)
-      e = kv_flash_launch<fmt(), true>(a, f, p.prefix_ct, dim3(a.kv_heads * p.prefix_parts, p.prefix_groups), st);
-    if (e == hipSuccess)
-      e = kv_flash_launch<fmt(), false>(a, f, p.own_ct, dim3(a.kv_heads * p.own_parts, p.own_groups, a.batch), st);
+    constexpr int FMT = fmt(), MOST = FMT == LFM_KV_F32 ? 2 : 4;
+    hipError_t e = by_columns<MOST>(p.own_ct, [&](auto own) -> hipError_t {
+      constexpr int CT = own();
+      if (!p.prefix_parts)
+        hipLaunchKernelGGL((kv_flash_kernel<FMT, CT>), dim3(a.kv_heads * p.own_parts, p.own_groups, a.batch),
+                           dim3(64 * own_waves(CT)), 0, st, a, f);
+      else if (p.prefix_ct == 1)
+        hipLaunchKernelGGL((kv_prefix_flash_kernel<FMT, 1, CT < 1 ? CT : 1>), dim3((unsigned)(prefix_blocks + own_blocks)),
+                           dim3(256), 0, st, a, f, (int)prefix_blocks, p.own_groups);
+      else
+        hipLaunchKernelGGL((kv_prefix_flash_kernel<FMT, MOST, CT>), dim3((unsigned)(prefix_blocks + own_blocks)),
+                           dim3(256), 0, st, a, f, (int)prefix_blocks, p.own_groups);
+      return hipGetLastError();
+    });
     if (e == hipSuccess && p.own_parts + p.prefix_parts > 1) {
       hipLaunchKernelGGL(kv_join_kernel, dim3((unsigned)((a.max_new * (long long)heads + 3) / 4), a.batch), dim3(256), 0,
                          st, a, f);
