@@ -423,19 +423,33 @@ __device__ __forceinline__ void flash_part(const KvArgs &a, const FlashArgs &f, 
       const int k0 = min(t * kKeys + 16 * hb, (len - 1) & ~15), page = hb ? page1 : page0;
       r.ok[hb] = page >= 0;
       const size_t row = kv_row(a, max(page, 0), h, k0 & ((1 << a.pshift) - 1));
-      const char *kp = a.k + row * kRowDim * kv_size<FMT>(), *vp = a.v + row * kRowDim * kv_size<FMT>();
+      // the half tile's 16 rows as buffers: a scalar base, and offsets of the lane alone
+      constexpr int kRowBytes = kRowDim * kv_size<FMT>(), kBytes = 16 * kRowBytes;
+      const auto kr = __builtin_amdgcn_make_buffer_rsrc(a.k + row * kRowBytes, 0, kBytes, moe::kBufferRsrcWord3);
+      const auto vr = __builtin_amdgcn_make_buffer_rsrc(a.v + row * kRowBytes, 0, kBytes, moe::kBufferRsrcWord3);
 #pragma unroll
       for (int w = 0; w < Raw::KW; ++w)
-        r.k[hb][w] = *reinterpret_cast<const u32x4 *>(kp + c * kRowDim * kv_size<FMT>() + 64 * w + 16 * g);
+        r.k[hb][w] = __builtin_amdgcn_raw_buffer_load_b128(kr, c * kRowBytes + 16 * g + 64 * w, 0, 0);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const uint32_t *p = reinterpret_cast<const uint32_t *>(vp + ((4 * g + i) * kRowDim + 4 * c) * kv_size<FMT>());
+        const int at = (4 * g + i) * kRowBytes + 4 * c * kv_size<FMT>();
+        if constexpr (Raw::KW == 1) {
+          r.v[hb][i][0] = __builtin_amdgcn_raw_buffer_load_b32(vr, at, 0, 0);
+        } else if constexpr (Raw::KW == 2) {
+          const auto x = __builtin_amdgcn_raw_buffer_load_b64(vr, at, 0, 0);
+          r.v[hb][i][0] = x[0];
+          r.v[hb][i][1] = x[1];
+        } else {
+          const auto x = __builtin_amdgcn_raw_buffer_load_b128(vr, at, 0, 0);
 #pragma unroll
-        for (int w = 0; w < Raw::KW; ++w) r.v[hb][i][w] = p[w];
+          for (int w = 0; w < 4; ++w) r.v[hb][i][w] = x[w];
+        }
       }
       if constexpr (Raw::SCALED) {
-        r.ks[hb] = moe::ld4(a.ks + row + 4 * g);
-        r.vs[hb] = moe::ld4(a.vs + row + 4 * g);
+        const auto ksr = __builtin_amdgcn_make_buffer_rsrc(a.ks + row, 0, 64, moe::kBufferRsrcWord3);
+        const auto vsr = __builtin_amdgcn_make_buffer_rsrc(a.vs + row, 0, 64, moe::kBufferRsrcWord3);
+        r.ks[hb] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(ksr, 16 * g, 0, 0));
+        r.vs[hb] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(vsr, 16 * g, 0, 0));
       }
     }
   };
@@ -455,73 +469,24 @@ __device__ __forceinline__ void flash_part(const KvArgs &a, const FlashArgs &f, 
     for (int d = 0; d < 4; ++d) o[ct][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   }
 
-  // Tile t from r, which then takes tile `next`, on pages next0 and next1.
-  auto tile = [&](int t, Raw &r, int next, int next0, int next1) {
+  // Tile t from r, while `next` (on pages next0 and next1) is loaded to rn.  The
+  // values become operands after the scores, for the registers.
+  auto tile = [&](int t, Raw &r, Raw &rn, int next, int next0, int next1) {
     const int k0 = t * kKeys;
     const bool ok[2] = {r.ok[0], r.ok[1]};
     // some keys are behind the end, behind a column's own position or on no page (wave-uniform)
     const bool cut = k0 + kKeys > first_seen || !ok[0] || !ok[1];
-    f32x4 ks[2], vs[2];
-    bf16x8 kop[2][2][NP], vop[4][NP];
-    // A value that is not finite must not meet the zero weight of a column that
-    // does not see it: such values (a bit each in nf) leave the product and make
-    // the outputs of the columns that do see them NaN.
-    uint32_t nf = 0;
     if constexpr (Raw::SCALED) {
+      // or the compiler takes the bytes apart as they arrive, in three steps each
 #pragma unroll
-      for (int hb = 0; hb < 2; ++hb) {
-        ks[hb] = r.ks[hb];
-        vs[hb] = r.vs[hb];
-      }
+      for (int hb = 0; hb < 2; ++hb) asm("" : "+v"(r.k[hb][0]));
     }
-    if (cut) {  // values of keys behind the sequence's end or on no page: zero
-#pragma unroll
-      for (int hb = 0; hb < 2; ++hb)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const bool there = ok[hb] && k0 + 16 * hb + 4 * g + i < len;
-#pragma unroll
-          for (int w = 0; w < Raw::KW; ++w) r.v[hb][i][w] = there ? r.v[hb][i][w] : 0u;
-          if constexpr (Raw::SCALED) {
-            const float x = vs[hb][i];
-            const bool finite = PREFIX || __builtin_fabsf(x) <= __FLT_MAX__;  // all see the prefix
-            if (there && !finite) nf |= 0x01010101u << (4 * hb + i);
-            vs[hb][i] = there && finite ? x : 0.0f;
-          }
-        }
-    }
+    load(next, next0, next1, rn);
+    bf16x8 kop[2][2][NP];
 #pragma unroll
     for (int hb = 0; hb < 2; ++hb)
 #pragma unroll
       for (int st = 0; st < 2; ++st) key_operand<FMT>(r, hb, st, kop[hb][st]);
-    value_operands<FMT>(r, vop);
-    load(next, next0, next1, r);
-
-    bool apart = false;
-    if (!PREFIX && cut) {
-      if constexpr (FMT != LFM_KV_INT8) {
-#pragma unroll
-        for (int db = 0; db < 4; ++db) {
-          const u32x4 w = __builtin_bit_cast(u32x4, vop[db][0]);
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            nf |= ((w[j] & 0x7F80u) == 0x7F80u ? 1u : 0u) << (8 * db + 2 * j) |
-                  ((w[j] & 0x7F800000u) == 0x7F800000u ? 2u : 0u) << (8 * db + 2 * j);
-        }
-      }
-      apart = __any(nf != 0);
-      if (apart && FMT != LFM_KV_INT8) {
-#pragma unroll
-        for (int db = 0; db < 4; ++db)
-#pragma unroll
-          for (int q = 0; q < NP; ++q) {
-            u32x4 w = __builtin_bit_cast(u32x4, vop[db][q]);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) w[j] &= ~half_mask(nf >> (8 * db + 2 * j));
-            vop[db][q] = __builtin_bit_cast(bf16x8, w);
-          }
-      }
-    }
 
     // scores of keys 16 hb + 4g + i against the running maximum
     float p[NT][8];
@@ -538,7 +503,7 @@ __device__ __forceinline__ void flash_part(const KvArgs &a, const FlashArgs &f, 
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const float sc = FEW ? sum_parts(acc[i]) : (float)acc[i];
-          p[ct][4 * hb + i] = Raw::SCALED ? __builtin_fmaf(sc, ks[hb][i], -ref[ct]) : sc - ref[ct];
+          p[ct][4 * hb + i] = Raw::SCALED ? __builtin_fmaf(sc, r.ks[hb][i], -ref[ct]) : sc - ref[ct];
         }
       }
     }
@@ -585,13 +550,55 @@ __device__ __forceinline__ void flash_part(const KvArgs &a, const FlashArgs &f, 
         }
       }
     }
+    bf16x8 vop[4][NP];
+    value_operands<FMT>(r, vop);
+    // A value (or its row's scale) that is not finite must not meet the zero
+    // weight of a column that does not see it, nor what stands behind the end or
+    // on no page: such values (a bit each in nf) leave the product and make the
+    // outputs of the columns that do see them NaN.
+    uint32_t nf = 0;
+    bool apart = false;
+    if (cut) {
+      if constexpr (FMT != LFM_KV_INT8) {
+#pragma unroll
+        for (int db = 0; db < 4; ++db) {
+          const u32x4 w = __builtin_bit_cast(u32x4, vop[db][0]);
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            nf |= ((w[j] & 0x7F80u) == 0x7F80u ? 1u : 0u) << (8 * db + 2 * j) |
+                  ((w[j] & 0x7F800000u) == 0x7F800000u ? 2u : 0u) << (8 * db + 2 * j);
+        }
+      }
+      if constexpr (Raw::SCALED) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (!(__builtin_fabsf(r.vs[e >> 2][e & 3]) <= __FLT_MAX__)) nf |= 0x01010101u << e;
+      }
+      apart = __any(nf != 0);
+      if (apart) {
+#pragma unroll
+        for (int db = 0; db < 4; ++db)
+#pragma unroll
+          for (int q = 0; q < NP; ++q) {
+            u32x4 w = __builtin_bit_cast(u32x4, vop[db][q]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[j] &= ~half_mask(nf >> (8 * db + 2 * j));
+            vop[db][q] = __builtin_bit_cast(bf16x8, w);
+          }
+        if constexpr (Raw::SCALED) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) r.vs[e >> 2][e & 3] = nf >> e & 1u ? 0.0f : r.vs[e >> 2][e & 3];
+        }
+      }
+    }
+
 #pragma unroll
     for (int ct = 0; ct < NT; ++ct) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         p[ct][e] = __builtin_amdgcn_exp2f(p[ct][e]);
         l[ct] += p[ct][e];
-        if constexpr (Raw::SCALED) p[ct][e] *= vs[e >> 2][e & 3];
+        if constexpr (Raw::SCALED) p[ct][e] *= r.vs[e >> 2][e & 3];
       }
       bf16x8 pp[QP];
       if constexpr (FEW)
@@ -610,6 +617,7 @@ __device__ __forceinline__ void flash_part(const KvArgs &a, const FlashArgs &f, 
         for (int j = 0; j < 4; ++j) {
           const int k = k0 + 16 * (j >> 1) + 4 * g + 2 * (j & 1);
           see[j] = (k <= last[ct] ? 0x3F80u : 0u) | (k + 1 <= last[ct] ? 0x3F800000u : 0u);
+          see[j] = ok[j >> 1] ? see[j] : 0u;
         }
 #pragma unroll
         for (int d = 0; d < 4; ++d) {
@@ -626,13 +634,13 @@ __device__ __forceinline__ void flash_part(const KvArgs &a, const FlashArgs &f, 
     }
   };
 
-  Raw r;
+  Raw ra, rb;  // two tiles: one computed, one on its way
   int pages = 0;
   if (t0 < t_end) {
     pages = in_cache(page_of(t0));
     const int half0 = __builtin_amdgcn_readlane(first_pages, 0);
     const int half1 = t0 * kKeys + 16 < len ? __builtin_amdgcn_readlane(first_pages, 1) : half0;
-    load(t0, in_cache(half0), in_cache(half1), r);
+    load(t0, in_cache(half0), in_cache(half1), ra);
   }
   // q's parts, scaled so that a score is the log2 of its weight
 #pragma unroll
@@ -651,14 +659,20 @@ __device__ __forceinline__ void flash_part(const KvArgs &a, const FlashArgs &f, 
     }
   }
   __syncthreads();  // q's parts are there
-  for (int t = t0, n = 0; t < t_end; t += stride, ++n) {
-    // the next tile's loads set out once this one's are operands; behind the
-    // wave's last tile that one is loaded again (its lines are in L2)
+  int t = t0, n = 0;
+  // behind the wave's last tile that one is loaded again (its lines are in L2)
+  auto step = [&](Raw &r, Raw &rn) {
     const bool more = t + stride < t_end;
-    const int i = (n + (more ? 1 : 0)) & 31;
-    if (more && i == 0) pages = in_cache(page_of(t + stride));
-    tile(t, r, more ? t + stride : t, __builtin_amdgcn_readlane(pages, 2 * i),
-         __builtin_amdgcn_readlane(pages, 2 * i + 1));
+    const int next = more ? t + stride : t, i = (n + (more ? 1 : 0)) & 31;
+    if (more && i == 0) pages = in_cache(page_of(next));
+    tile(t, r, rn, next, __builtin_amdgcn_readlane(pages, 2 * i), __builtin_amdgcn_readlane(pages, 2 * i + 1));
+    t += stride;
+    ++n;
+  };
+  while (t < t_end) {
+    step(ra, rb);
+    if (t >= t_end) break;
+    step(rb, ra);
   }
   __syncthreads();  // and read for the last time
 
