@@ -853,20 +853,25 @@ hipError_t launch_kv_read(const KvArgs &a, float *k_out, float *v_out, int rows,
 }
 
 // How a call is split: column tiles a wave holds, and parts of the own positions
-// and of the prefix so that about as many blocks run as the CUs hold.
-constexpr int kOwnBlocks = 512, kOneTileBlocks = 1024, kPrefixBlocks = 256;
-
+// and of the prefix.  Parts are added where a wave has most to do, as long as the
+// blocks fit the CUs at once, since a second round of blocks begins with the same
+// chain of loads (6-8 us) as the first: 16 x 5 tokens of 1000 int8 positions behind
+// 2000 shared ones take 18.8 us in 416 blocks, 22.1 in 536, 24.5 in 792.  Where the
+// sequences alone fill the CUs the prefix gets half as many blocks beside them
+// (64 x 1 token behind 8192 fp8 positions: 34.9 us in 128 blocks, 24.3 in 256, 28.7
+// in 512).
 struct FlashPlan {
   int own_ct, prefix_ct, own_groups, prefix_groups, own_parts, prefix_parts;
 };
+
+constexpr int kFlashCUs = 256, kMostParts = 256;
 
 static int columns_of(int ct) { return ct == 0 ? kFewCols : 16 * ct; }
 
 static int widest(int format) { return format == LFM_KV_F32 ? 2 : 4; }
 
-static int parts_of(long long keys, long long blocks, long long want) {
-  return active_parts((int)keys, (int)std::min<long long>(std::max<long long>(1, (want + blocks - 1) / blocks), 256));
-}
+// A tile's time, to that of one column tile.
+static float tile_cost(int ct) { return ct <= 1 ? 1.0f : ct == 2 ? 1.6f : 2.8f; }
 
 static FlashPlan flash_plan(const KvArgs &a, int heads) {
   FlashPlan p{};
@@ -874,13 +879,30 @@ static FlashPlan flash_plan(const KvArgs &a, int heads) {
   const long long own = a.max_new * group, all = a.tokens * group;
   p.own_ct = own <= kFewCols ? 0 : own <= 16 ? 1 : std::min(widest(a.format), own <= 32 ? 2 : 4);
   p.own_groups = (int)((own + columns_of(p.own_ct) - 1) / columns_of(p.own_ct));
-  p.own_parts = parts_of(std::min<long long>(a.max_len ? a.max_len : cap, cap),
-                         (long long)p.own_groups * a.kv_heads * std::max(a.batch, 1),
-                         p.own_ct == 1 ? kOneTileBlocks : kOwnBlocks);
-  if (a.prefix_len > 0) {
-    p.prefix_ct = all <= 16 && p.own_ct <= 1 ? 1 : widest(a.format);
-    p.prefix_groups = (int)((all + columns_of(p.prefix_ct) - 1) / columns_of(p.prefix_ct));
-    p.prefix_parts = parts_of(a.prefix_len, (long long)p.prefix_groups * a.kv_heads, kPrefixBlocks);
+  p.own_parts = 1;
+  const int keys = (int)std::min<long long>(a.max_len ? a.max_len : cap, cap);
+  const long long own_base = (long long)p.own_groups * a.kv_heads * std::max(a.batch, 1);
+  const int most = active_parts(keys, kMostParts);
+  const float own_time = (float)keys * tile_cost(p.own_ct);  // of a wave
+  if (a.prefix_len == 0) {
+    const long long slots = kFlashCUs * flash_waves(a.format, p.own_ct) * 4 / own_waves(p.own_ct);
+    p.own_parts = (int)std::min<long long>(most, std::max<long long>(1, slots / own_base));
+    return p;
+  }
+  p.prefix_ct = all <= 16 && p.own_ct <= 1 ? 1 : widest(a.format);
+  p.prefix_groups = (int)((all + columns_of(p.prefix_ct) - 1) / columns_of(p.prefix_ct));
+  p.prefix_parts = 1;
+  const long long prefix_base = (long long)p.prefix_groups * a.kv_heads;
+  const int prefix_most = active_parts(a.prefix_len, kMostParts);
+  const float prefix_time = (float)a.prefix_len * tile_cost(p.prefix_ct);
+  const long long slots = kFlashCUs * flash_waves(a.format, p.prefix_ct);
+  const long long budget = std::max(slots, own_base + slots / 2);
+  for (;;) {
+    const bool prefix = prefix_time * p.own_parts >= own_time * p.prefix_parts;
+    int &parts = prefix ? p.prefix_parts : p.own_parts;
+    if (parts >= (prefix ? prefix_most : most)) break;
+    if (own_base * p.own_parts + prefix_base * p.prefix_parts + (prefix ? prefix_base : own_base) > budget) break;
+    ++parts;
   }
   return p;
 }
