@@ -16,7 +16,16 @@ namespace lfm {
 // ---------------------------------------------------------------------------
 
 // 16 lanes take a row of 64 (a token's q, k or v head), four floats each, R rows
-// one after the other with their loads in flight together; block (x, sequence).
+// one after the other; block (x, sequence).  Every load that hangs on nothing but
+// the sequence stands in front, without a branch: pages, then rows.
+
+// The page of own position pos of sequence b; -1 (and the flag) outside the cache.
+__device__ __forceinline__ int kv_page(const KvArgs &a, int page) {
+  if (page >= 0 && page < a.num_pages) return page;
+  kv_flag(a.bad);
+  return -1;
+}
+
 template <int FMT, bool ROPE, int R>
 __global__ __launch_bounds__(256) void kv_write_kernel(KvArgs a, KvWriteArgs w) {
   KvSeq s;
@@ -25,18 +34,29 @@ __global__ __launch_bounds__(256) void kv_write_kernel(KvArgs a, KvWriteArgs w) 
   const int first = blockIdx.x * 16 * R;
   if (first >= total) return;
   const int c = threadIdx.x & 15, g = threadIdx.x >> 4;
-  f32x4 x[R];
-  int tok[R], row[R];
+  f32x4 x[R], cs[R], sn[R];
+  int tok[R], row[R], page[R];
 #pragma unroll
   for (int j = 0; j < R; ++j) {
-    const int f = first + 16 * j + g;
+    const int f = min(first + 16 * j + g, total - 1);  // a surplus row repeats the last, and is not stored
     tok[j] = f / per_tok;
     row[j] = f - tok[j] * per_tok;
+    const int pos = s.len - s.n + tok[j];
+    page[j] = a.pages[(size_t)blockIdx.y * a.max_pages + (pos >> a.pshift)];
     const int col = row[j] < qrows ? row[j] * kRowDim
                     : row[j] < qrows + a.kv_heads ? w.k_col + (row[j] - qrows) * kRowDim
                                                   : w.v_col + (row[j] - qrows - a.kv_heads) * kRowDim;
-    x[j] = f < total ? moe::ld4(w.qkv + (size_t)(s.row0 + tok[j]) * w.ld + col + 4 * c)
-                     : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    x[j] = moe::ld4(w.qkv + (size_t)(s.row0 + tok[j]) * w.ld + col + 4 * c);
+    if (ROPE) {
+      const size_t t = (size_t)min(a.prefix_len + pos, w.max_pos - 1) * kRowDim + 4 * c;
+      cs[j] = moe::ld4(w.cos_t + t);
+      sn[j] = moe::ld4(w.sin_t + t);
+    }
+  }
+  f32x4 wq, wk;
+  if (ROPE) {
+    wq = moe::ld4(w.q_weight + 4 * c);
+    wk = moe::ld4(w.k_weight + 4 * c);
   }
 #pragma unroll
   for (int j = 0; j < R; ++j) {
@@ -44,25 +64,18 @@ __global__ __launch_bounds__(256) void kv_write_kernel(KvArgs a, KvWriteArgs w) 
     const int pos = s.len - s.n + tok[j];
     const bool is_q = row[j] < qrows, is_v = row[j] >= qrows + a.kv_heads;
     if (ROPE) {
-      const int at = a.prefix_len + pos;
-      if (ok && at >= w.max_pos) {
+      if (ok && a.prefix_len + pos >= w.max_pos) {
         kv_flag(a.bad);
         ok = false;
       }
-      const size_t t = (size_t)(ok ? at : 0) * kRowDim + 4 * c;
-      const f32x4 y = norm_rope_row(x[j], moe::ld4((is_q ? w.q_weight : w.k_weight) + 4 * c),
-                                    moe::ld4(w.cos_t + t), moe::ld4(w.sin_t + t));
+      const f32x4 y = norm_rope_row(x[j], is_q ? wq : wk, cs[j], sn[j]);
       if (!is_v) x[j] = y;
       if (ok && is_q) moe::st4(w.qkv + (size_t)(s.row0 + tok[j]) * w.ld + row[j] * kRowDim + 4 * c, y);
     }
     const int h = row[j] - qrows - (is_v ? a.kv_heads : 0);
     ok = ok && !is_q;
-    const int page = ok ? a.pages[(size_t)blockIdx.y * a.max_pages + (pos >> a.pshift)] : 0;
-    if (page < 0 || page >= a.num_pages) {
-      kv_flag(a.bad);
-      ok = false;
-    }
-    const size_t at = ok ? kv_row(a, page, h, pos & ((1 << a.pshift) - 1)) : 0;
+    if (ok) ok = kv_page(a, page[j]) >= 0;
+    const size_t at = ok ? kv_row(a, page[j], h, pos & ((1 << a.pshift) - 1)) : 0;
     kv_store_row<FMT>(is_v ? a.v : a.k, is_v ? a.vs : a.ks, at, c, x[j], ok);
   }
 }
@@ -75,29 +88,29 @@ __global__ __launch_bounds__(256) void kv_read_kernel(KvArgs a, float *k_out, fl
   const int total = min(s.len, rows) * per_pos, first = blockIdx.x * 16 * R;
   if (first >= total) return;
   const int c = threadIdx.x & 15, g = threadIdx.x >> 4;
+  int pos[R], row[R], page[R];
+#pragma unroll
+  for (int j = 0; j < R; ++j) {
+    const int f = min(first + 16 * j + g, total - 1);  // a surplus row repeats the last
+    pos[j] = f / per_pos;
+    row[j] = f - pos[j] * per_pos;
+    page[j] = a.pages[(size_t)blockIdx.y * a.max_pages + (pos[j] >> a.pshift)];
+  }
   f32x4 x[R];
 #pragma unroll
   for (int j = 0; j < R; ++j) {
-    const int f = first + 16 * j + g, pos = f / per_pos, row = f - pos * per_pos;
-    x[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    if (f >= total) continue;
-    const bool is_v = !k_out || row >= a.kv_heads;
-    const int page = a.pages[(size_t)blockIdx.y * a.max_pages + (pos >> a.pshift)];
-    if (page < 0 || page >= a.num_pages) {
-      kv_flag(a.bad);
-      continue;
-    }
-    const size_t at = kv_row(a, page, row >= a.kv_heads ? row - a.kv_heads : row, pos & ((1 << a.pshift) - 1));
+    page[j] = kv_page(a, page[j]);
+    const bool is_v = !k_out || row[j] >= a.kv_heads;
+    const size_t at = kv_row(a, max(page[j], 0), row[j] >= a.kv_heads ? row[j] - a.kv_heads : row[j],
+                             pos[j] & ((1 << a.pshift) - 1));
     x[j] = kv_load_row<FMT>(is_v ? a.v : a.k, is_v ? a.vs : a.ks, at, c);
   }
 #pragma unroll
   for (int j = 0; j < R; ++j) {
-    const int f = first + 16 * j + g, pos = f / per_pos, row = f - pos * per_pos;
-    if (f >= total) continue;
-    const bool is_v = !k_out || row >= a.kv_heads;
-    float *o = is_v ? v_out : k_out;
-    moe::st4(o + ((size_t)blockIdx.y * rows + pos) * ld + (row >= a.kv_heads ? row - a.kv_heads : row) * kRowDim +
-                 4 * c, x[j]);
+    const bool is_v = !k_out || row[j] >= a.kv_heads;
+    float *o = (is_v ? v_out : k_out) + ((size_t)blockIdx.y * rows + pos[j]) * ld +
+               (row[j] >= a.kv_heads ? row[j] - a.kv_heads : row[j]) * kRowDim + 4 * c;
+    if (first + 16 * j + g < total) moe::st4(o, page[j] >= 0 ? x[j] : f32x4{0.0f, 0.0f, 0.0f, 0.0f});
   }
 }
 
@@ -814,20 +827,28 @@ __global__ __launch_bounds__(256) void kv_join_kernel(KvArgs a, FlashArgs f) {
 // Launchers
 // ---------------------------------------------------------------------------
 
+// Rows a group of 16 lanes takes: four where they fill the CUs, else one.
+constexpr long long kSplitRows = 32768;
+
 template <int FMT, bool ROPE>
 static hipError_t kv_write_launch(const KvArgs &a, const KvWriteArgs &w, hipStream_t st) {
   const int rows = a.max_new * ((ROPE ? w.heads : 0) + 2 * a.kv_heads);
-  hipLaunchKernelGGL((kv_write_kernel<FMT, ROPE, 4>), dim3((rows + 63) / 64, a.batch), dim3(256), 0, st, a, w);
+  if ((long long)rows * a.batch <= kSplitRows)
+    hipLaunchKernelGGL((kv_write_kernel<FMT, ROPE, 1>), dim3((rows + 15) / 16, a.batch), dim3(256), 0, st, a, w);
+  else
+    hipLaunchKernelGGL((kv_write_kernel<FMT, ROPE, 4>), dim3((rows + 63) / 64, a.batch), dim3(256), 0, st, a, w);
   return hipGetLastError();
 }
 
 template <int FMT>
 static hipError_t kv_read_launch(const KvArgs &a, float *k_out, float *v_out, int rows, int ld, hipStream_t st) {
-  const int n = std::min<long long>(rows, (long long)a.max_pages << a.pshift) *
+  const int n = (int)std::min<long long>(rows, (long long)a.max_pages << a.pshift) *
                 ((k_out != nullptr) + (v_out != nullptr)) * a.kv_heads;
   if (n == 0) return hipSuccess;
-  hipLaunchKernelGGL((kv_read_kernel<FMT, 4>), dim3((n + 63) / 64, a.batch), dim3(256), 0, st, a, k_out, v_out, rows,
-                     ld);
+  if ((long long)n * a.batch <= kSplitRows)
+    hipLaunchKernelGGL((kv_read_kernel<FMT, 1>), dim3((n + 15) / 16, a.batch), dim3(256), 0, st, a, k_out, v_out, rows, ld);
+  else
+    hipLaunchKernelGGL((kv_read_kernel<FMT, 4>), dim3((n + 63) / 64, a.batch), dim3(256), 0, st, a, k_out, v_out, rows, ld);
   return hipGetLastError();
 }
 
