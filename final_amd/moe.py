@@ -20,16 +20,16 @@ TOPK = 4
 
 def _ptr(x):
     """int pointer from a DeviceArray, an int or None."""
-    if x is None:
-        return None
+    if x is None or type(x) is int:
+        return x
     if isinstance(x, hip.DeviceArray):
         return x.ptr
     return int(x)
 
 
 def _stream(s):
-    if s is None:
-        return None
+    if s is None or type(s) is int:
+        return s
     if isinstance(s, hip.Stream):
         return s.ptr
     return int(s)
