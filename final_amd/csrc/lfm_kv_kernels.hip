@@ -878,14 +878,15 @@ hipError_t launch_kv_read(const KvArgs &a, float *k_out, float *v_out, int rows,
 // blocks fit the CUs at once, since a second round of blocks begins with the same
 // chain of loads (6-8 us) as the first: 16 x 5 tokens of 1000 int8 positions behind
 // 2000 shared ones take 18.8 us in 416 blocks, 22.1 in 536, 24.5 in 792.  Where the
-// sequences alone fill the CUs the prefix gets half as many blocks beside them
-// (64 x 1 token behind 8192 fp8 positions: 34.9 us in 128 blocks, 24.3 in 256, 28.7
-// in 512).
+// sequences alone fill the CUs the prefix gets half as many blocks beside them, or
+// as many where it is longer than kLongPrefix (64 x 1 token behind fp8 positions, us
+// in 256 / 512 blocks: 8192 23.9 / 27.8, 16384 37.0 / 39.4, 32768 63.6 / 58.0; 8192
+// in 128: 34.9).
 struct FlashPlan {
   int own_ct, prefix_ct, own_groups, prefix_groups, own_parts, prefix_parts;
 };
 
-constexpr int kFlashCUs = 256, kMostParts = 256;
+constexpr int kFlashCUs = 256, kMostParts = 256, kLongPrefix = 20480;
 
 static int columns_of(int ct) { return ct == 0 ? kFewCols : 16 * ct; }
 
@@ -917,7 +918,7 @@ static FlashPlan flash_plan(const KvArgs &a, int heads) {
   const int prefix_most = active_parts(a.prefix_len, kMostParts);
   const float prefix_time = (float)a.prefix_len * tile_cost(p.prefix_ct);
   const long long slots = kFlashCUs * flash_waves(a.format, p.prefix_ct);
-  const long long budget = std::max(slots, own_base + slots / 2);
+  const long long budget = std::max(slots, own_base + (a.prefix_len > kLongPrefix ? slots : slots / 2));
   for (;;) {
     const bool prefix = prefix_time * p.own_parts >= own_time * p.prefix_parts;
     int &parts = prefix ? p.prefix_parts : p.own_parts;
