@@ -97,12 +97,14 @@ __device__ __forceinline__ void load_values(const float *x, int n, float (&v)[NR
   }
 }
 
+// Groups [j0, j1) of a thread's values.
 template <int NW, int NR, int VEC>
-__device__ __forceinline__ void store_values(float *y, int n, const float (&v)[NR], float scale) {
+__device__ __forceinline__ void store_values(float *y, int n, const float (&v)[NR], float scale, int j0 = 0,
+                                             int j1 = NR / VEC) {
 #pragma unroll
   for (int j = 0; j < NR / VEC; ++j) {
     const int i = (j * NW * 64 + (int)threadIdx.x) * VEC;
-    if (i >= n) continue;
+    if (i >= n || j < j0 || j >= j1) continue;
     if (VEC == 4) {
       moe::st4(y + i, f32x4{v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]} * scale);
     } else {
@@ -113,7 +115,8 @@ __device__ __forceinline__ void store_values(float *y, int n, const float (&v)[N
 
 __device__ __forceinline__ float inverse_sum(float l) { return l == 0.0f ? 0.0f : 1.0f / l; }
 
-// A row a block, NR values a thread.
+// A row, NR values a thread; gridDim.y blocks each read all of it and write their
+// share.
 template <int NR, int VEC>
 __global__ __launch_bounds__(kSoftThreads) __attribute__((amdgpu_waves_per_eu(NR <= 32 ? 8 : 4)))
 void softmax_row_kernel(const float *x, long long xs, float *y, long long ys,
@@ -125,7 +128,8 @@ void softmax_row_kernel(const float *x, long long xs, float *y, long long ys,
   float v[NR];
   load_values<NW, NR, VEC>(x, dim, v);
   const MaxSum r = block_exp<NW, NR>(v, c, s_part);
-  store_values<NW, NR, VEC>(y, dim, v, inverse_sum(r.l));
+  const int share = NR / VEC / gridDim.y;
+  store_values<NW, NR, VEC>(y, dim, v, inverse_sum(r.l), blockIdx.y * share, (blockIdx.y + 1) * share);
 }
 
 // A slice of a row a block: its maximum and sum.
@@ -163,17 +167,28 @@ __global__ __launch_bounds__(kSliceThreads) void softmax_finish_kernel(const flo
   store_values<NW, kSliceRegs, VEC>(y + blockIdx.y * ys + first, n, v, inv);
 }
 
-// How many of the first rows are taken whole.  Short ones all are (8192 values:
-// one launch, 5 us); of rows up to kSoftRow values, of which a CU holds one or
-// two, full rounds of the CUs and a last one that is kSoftMost of a round: a
-// round of 65536 values takes 27 us, kSoftMost of it split as long.
-constexpr int kShortRow = 8 * kSoftThreads, kSoftCUs = 256;
+// How many of the first rows take a block each.  Those of up to 8192 values all do;
+// of 32768, of which a CU holds two, from 128 rows; of 65536, of which it holds one,
+// full rounds of the CUs and a last one from 144 rows (65536 values, a block a row /
+// split: 128 rows 16.3 / 16.8 us, 160 rows 17.7 / 23.2, 256 rows 25.6 / 36).
+constexpr int kShortRow = 8 * kSoftThreads, kMidRow = 32 * kSoftThreads, kSoftCUs = 256;
 
 static int whole_rows(int rows, int dim) {
   if (dim <= kShortRow) return rows;
   if (dim > kSoftRow) return 0;
-  const int round = dim <= 32 * kSoftThreads ? 2 * kSoftCUs : kSoftCUs, left = rows % round;
-  return left >= round / 4 * 3 ? rows : rows - left;
+  if (dim <= kMidRow) return rows >= 128 ? rows : 0;
+  const int left = rows % kSoftCUs;
+  return left >= 144 ? rows : rows - left;
+}
+
+// Whether the others share the CUs' blocks out between them, each block reading a
+// whole row, where nobody overwrites what another has to read (y is not x): one
+// launch instead of two (1 row of 65536: 8.0 us, split 6.5 and a launch; 64 rows of
+// 32000: 7.8 / 8.2; 64 rows of 65536 from HBM 18 / 12).
+constexpr int kShareRows = 32;
+
+static bool share_rows(int left, int whole, int dim) {
+  return dim <= kMidRow || (dim <= kSoftRow && whole == 0 && left <= kShareRows);
 }
 
 size_t softmax_ws(int rows, int dim) {
@@ -181,22 +196,35 @@ size_t softmax_ws(int rows, int dim) {
 }
 
 template <int VEC>
+static void softmax_rows_launch(const float *x, long long xs, float *y, long long ys, int rows, int share, int dim,
+                                float c, hipStream_t st) {
+  const dim3 grid(rows, share), block(kSoftThreads);
+  if (dim <= kShortRow)
+    hipLaunchKernelGGL((softmax_row_kernel<8, VEC>), grid, block, 0, st, x, xs, y, ys, dim, c);
+  else if (dim <= kMidRow)
+    hipLaunchKernelGGL((softmax_row_kernel<32, VEC>), grid, block, 0, st, x, xs, y, ys, dim, c);
+  else
+    hipLaunchKernelGGL((softmax_row_kernel<64, VEC>), grid, block, 0, st, x, xs, y, ys, dim, c);
+}
+
+template <int VEC>
 static hipError_t softmax_launch(const float *x, long long xs, float *y, long long ys, int rows, int dim, float c,
                                  void *ws, hipStream_t st) {
-  const int whole = whole_rows(rows, dim);
-  if (whole > 0) {
-    if (dim <= 8 * kSoftThreads)
-      hipLaunchKernelGGL((softmax_row_kernel<8, VEC>), dim3(whole), dim3(kSoftThreads), 0, st, x, xs, y, ys, dim, c);
-    else if (dim <= 32 * kSoftThreads)
-      hipLaunchKernelGGL((softmax_row_kernel<32, VEC>), dim3(whole), dim3(kSoftThreads), 0, st, x, xs, y, ys, dim, c);
-    else
-      hipLaunchKernelGGL((softmax_row_kernel<64, VEC>), dim3(whole), dim3(kSoftThreads), 0, st, x, xs, y, ys, dim, c);
+  const int whole = whole_rows(rows, dim), left = rows - whole;
+  if (whole > 0) softmax_rows_launch<VEC>(x, xs, y, ys, whole, 1, dim, c, st);
+  x += whole * xs;
+  y += whole * ys;
+  if (left > 0 && x != y && share_rows(left, whole, dim)) {
+    int share = 1;
+    while (share < 8 && 2 * share * left <= kSoftCUs) share *= 2;
+    softmax_rows_launch<VEC>(x, xs, y, ys, left, share, dim, c, st);
+    return hipGetLastError();
   }
   const int slices = (dim + kSlice - 1) / kSlice;
   float2 *part = static_cast<float2 *>(ws);
-  for (int r0 = whole; r0 < rows; r0 += 65535) {  // rows a launch may have
-    const dim3 grid(slices, std::min(rows - r0, 65535));
-    float2 *p = part + (size_t)(r0 - whole) * slices;
+  for (int r0 = 0; r0 < left; r0 += 65535) {  // rows a launch may have
+    const dim3 grid(slices, std::min(left - r0, 65535));
+    float2 *p = part + (size_t)r0 * slices;
     hipLaunchKernelGGL((softmax_part_kernel<VEC>), grid, dim3(kSliceThreads), 0, st, x + r0 * xs, xs, p, dim, c);
     hipLaunchKernelGGL((softmax_finish_kernel<VEC>), grid, dim3(kSliceThreads), 0, st, x + r0 * xs, xs, y + r0 * ys, ys, p,
                        dim, c);

@@ -193,8 +193,10 @@ int lfm_kv_attention_workspace(const lfm_kv_cache *cache, const lfm_kv_batch *ba
 /* y[r][i] = exp((x[r][i] - max x[r]) / temperature) / sum: probabilities of the
  * logits of `rows` rows of `dim`, row r at x + r*x_stride and y + r*y_stride
  * (floats).  A logit of -infinity gives 0, a row of nothing else zeros; NaN or
- * +infinity makes its row NaN.  temperature > 0.  y may be x (with equal
- * strides); otherwise the two do not overlap. */
+ * +infinity makes its row NaN.  temperature from 2^-120 to 2^120.  y may be
+ * x (with equal strides; the sums may then be taken in another order); otherwise
+ * the two do not overlap.  workspace: lfm_softmax_workspace bytes, as for
+ * lfm_kv_attention. */
 int lfm_softmax(const float *x, long long x_stride, float *y, long long y_stride, int rows, int dim,
                 float temperature, void *workspace, size_t workspace_bytes, moe_stream_t stream);
 int lfm_softmax_workspace(int rows, int dim, size_t *bytes);
@@ -210,10 +212,12 @@ int lfm_softmax_workspace(int rows, int dim, size_t *bytes);
  * that has no positive sum; after n_valid accepted drafts from target[n_valid].
  * It is the lowest id up to which the weights' sum exceeds u_sample times their
  * whole sum, in 64 bits; -1 where no weight is positive.  Weights that are NaN
- * or below 0 count as 0, and an id outside [0, vocab) is rejected.
+ * or below 0 count as 0 (an infinite one leaves -1), and an id outside [0, vocab)
+ * is rejected.
  * accepted [batch] = the number of accepted drafts; tokens [batch][n_draft + 1]
  * = these, the drawn token, then -1.  n_draft = 0 draws one token from target
- * (draft, draft_ids and u_accept may then be NULL). */
+ * (draft, draft_ids and u_accept may then be NULL).  n_draft at most 1024.
+ * workspace: lfm_verify_draft_workspace bytes, as for lfm_kv_attention. */
 int lfm_verify_draft(const float *target, const float *draft, const int *draft_ids,
                      const float *u_accept, const float *u_sample, const int *n_valid, int batch,
                      int n_draft, int vocab, int *accepted, int *tokens, void *workspace,
