@@ -36,7 +36,7 @@ LFM_SYMBOLS = (
     "lfm_verify_draft_workspace", "lfm_rope_tables", "lfm_synth_normal", "lfm_fill", "lfm_synth_stream_of",
     "lfm_synth_is_norm", "lfm_synth_tensor", "lfm_model_create_synthetic",
     "lfm_model_create_from_file", "lfm_model_destroy", "lfm_model_forward", "lfm_model_embed",
-    "lfm_model_layer_forward", "lfm_model_head", "lfm_model_moe", "lfm_model_info",
+    "lfm_model_layer_forward", "lfm_model_head", "lfm_model_verify", "lfm_model_moe", "lfm_model_info",
     "lfm_model_status",
 )
 SYNTH_SYMBOLS = (
@@ -143,7 +143,8 @@ def lib() -> ctypes.CDLL:
     L.lfm_kv_attention_workspace.argtypes = [_vp, _vp, _i, ctypes.POINTER(_sz)]
     L.lfm_softmax.argtypes = [_vp, _ll, _vp, _ll, _i, _i, _f, _vp, _sz, _vp]
     L.lfm_softmax_workspace.argtypes = [_i, _i, ctypes.POINTER(_sz)]
-    L.lfm_verify_draft.argtypes = [_vp] * 6 + [_i, _i, _i, _vp, _vp, _vp, _sz, _vp]
+    L.lfm_verify_draft.argtypes = [_vp, _vp, _vp, _ll, _vp, _vp, _vp, _i, _i, _i, _vp, _vp, _vp,
+                                   _sz, _vp]
     L.lfm_verify_draft_workspace.argtypes = [_i, _i, ctypes.POINTER(_sz)]
     L.lfm_rope_tables.argtypes = [_vp, _vp, _i, _i, _f]
     L.lfm_synth_normal.argtypes = [_vp, _sz, _u64, _u64, _f, _u64, _vp]
@@ -159,6 +160,7 @@ def lib() -> ctypes.CDLL:
     L.lfm_model_embed.argtypes = [_vp, _vp, _i, _i, _vp, _vp]
     L.lfm_model_layer_forward.argtypes = [_vp, _i, _vp, _i, _i, _vp]
     L.lfm_model_head.argtypes = [_vp, _vp, _i, _i, _vp, _vp]
+    L.lfm_model_verify.argtypes = [_vp, _vp, _i, _i, _i, _vp, _vp, _vp, _vp, _f, _vp, _vp, _vp, _vp]
     L.lfm_model_moe.argtypes = [_vp, _i, ctypes.POINTER(_vp)]
     L.lfm_model_info.argtypes = [_vp, ctypes.POINTER(_i), ctypes.POINTER(_i), ctypes.POINTER(_i),
                                  ctypes.POINTER(_i)]

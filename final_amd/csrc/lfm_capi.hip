@@ -233,19 +233,20 @@ int lfm_verify_draft_workspace(int batch, int vocab, size_t *bytes) {
 }
 
 int lfm_verify_draft(const float *target, const float *draft, const int *draft_ids,
-                     const float *u_accept, const float *u_sample, const int *n_valid, int batch,
+                     long long ids_stride, const float *u_accept, const float *u_sample, const int *n_valid, int batch,
                      int n_draft, int vocab, int *accepted, int *tokens, void *workspace,
                      size_t workspace_bytes, moe_stream_t stream) {
   if (batch < 0 || n_draft < 0 || vocab <= 0) return MOE_ERR_INVALID_ARG;
   if (batch == 0) return MOE_OK;
   if (batch > 65535 || n_draft > 1024) return MOE_ERR_UNSUPPORTED;
   if (!target || !u_sample || !accepted || !tokens) return MOE_ERR_INVALID_ARG;
-  if (n_draft > 0 && (!draft || !draft_ids || !u_accept)) return MOE_ERR_INVALID_ARG;
+  if (n_draft > 0 && (!draft || !draft_ids || !u_accept || ids_stride < n_draft))
+    return MOE_ERR_INVALID_ARG;
   const size_t need = lfm::verify_draft_ws(batch, vocab);
   if (need && (!workspace || !al16(workspace) || workspace_bytes < need)) return MOE_ERR_INVALID_ARG;
   return launch_status(lfm::launch_verify_draft(
       lfm::VerifyArgs{target, draft, draft_ids, u_accept, u_sample, n_valid, accepted, tokens, batch,
-                      n_draft, vocab},
+                      n_draft, vocab, ids_stride},
       workspace, S(stream)));
 }
 

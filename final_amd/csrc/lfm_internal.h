@@ -82,6 +82,7 @@ struct VerifyArgs {
   const int *n_valid;
   int *accepted, *tokens;
   int batch, n_draft, vocab;
+  long long ids_stride;
 };
 size_t verify_draft_ws(int batch, int vocab);
 hipError_t launch_verify_draft(const VerifyArgs &a, void *ws, hipStream_t st);

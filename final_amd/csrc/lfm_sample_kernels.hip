@@ -264,7 +264,7 @@ __device__ __forceinline__ int accepted_drafts(const VerifyArgs &a, int b, int n
     bool ok = i < a.n_draft;
     if (ok) {
       const size_t at = (size_t)b * a.n_draft + i;
-      const int id = a.ids[at];
+      const int id = a.ids[b * a.ids_stride + i];
       const float u = a.u_accept[at];
       ok = id >= 0 && id < a.vocab;
       if (ok) {
@@ -378,7 +378,7 @@ __global__ __launch_bounds__(kTokenThreads) void draw_token_kernel(VerifyArgs a,
   const int acc = a.accepted[b];
   const float u = a.u_sample[b];
   const int n = drafts_of(a, b);  // every load that hangs on nothing stands in front
-  const int id = tid < a.n_draft ? a.ids[(size_t)b * a.n_draft + tid] : -1;
+  const int id = tid < a.n_draft ? a.ids[b * a.ids_stride + tid] : -1;
   sums += (size_t)b * slices;
   // lane l holds the sums of `each` neighbouring slices
   const int each = (slices + 63) / 64, i0 = lane * each, i1 = min(i0 + each, slices);

@@ -148,6 +148,38 @@ void LFM2Model::head_gpu(const float *h, int batch, int seq_len, float *logits, 
         "lfm_gemm_nt lm_head");
 }
 
+void LFM2Model::verify_gpu(const int *ids, int batch, int seq_len, int n_draft, const float *draft,
+                           const float *u_accept, const float *u_sample, const int *n_valid,
+                           float temperature, float *probs, int *accepted, int *tokens,
+                           hipStream_t stream) {
+  check_shape(batch, seq_len);
+  if (n_draft < 0 || (seq_len > 0 && n_draft >= seq_len))
+    throw std::invalid_argument("LFM2Model::verify: n_draft");
+  if (!(temperature >= 0x1p-120f && temperature <= 0x1p120f))
+    throw std::invalid_argument("LFM2Model::verify: temperature");
+  if (batch == 0 || seq_len == 0) return;
+  embed_gpu(ids, batch, seq_len, hidden_, stream);
+  for (int i = 0; i < num_layers(); ++i) layer_forward_gpu(i, hidden_, batch, seq_len, stream);
+  // The layers are done with the workspace: the positions' norms go to its
+  // first buffer, the samplers' scratch (200 bytes a row) to its widest.
+  const long long H = (long long)HIDDEN_SIZE;
+  const int per = n_draft + 1, rows = batch * per;
+  for (int i = 0; i < per; ++i)
+    check(lfm_rmsnorm(hidden_ + (size_t)(seq_len - per + i) * H, (long long)seq_len * H,
+                      norm_->weight_gpu(), ws_->normed + i * H, (long long)per * H, batch, (int)H, stream),
+          "lfm_rmsnorm");
+  const float *head = lm_head_.size() ? lm_head_.gpu() : embed_tokens_.gpu();
+  check(lfm_gemm_nt(ws_->normed, head, probs, nullptr, rows, (int)vocab_, (int)H, stream),
+        "lfm_gemm_nt lm_head");
+  const size_t scratch = (size_t)batch * seq_len * 3 * H * sizeof(float);
+  check(lfm_softmax(probs, (long long)vocab_, probs, (long long)vocab_, rows, (int)vocab_, temperature,
+                    ws_->proj, scratch, stream),
+        "lfm_softmax");
+  check(lfm_verify_draft(probs, draft, ids + seq_len - n_draft, seq_len, u_accept, u_sample, n_valid,
+                         batch, n_draft, (int)vocab_, accepted, tokens, ws_->proj, scratch, stream),
+        "lfm_verify_draft");
+}
+
 void LFM2Model::forward_gpu(const int *ids, int batch, int seq_len, float *logits,
                             hipStream_t stream) {
   check_shape(batch, seq_len);
@@ -311,6 +343,20 @@ int lfm_model_head(lfm_model *m, const float *h, int batch, int seq, float *logi
                    moe_stream_t stream) {
   if (!m || (batch * seq > 0 && (!h || !logits))) return MOE_ERR_INVALID_ARG;
   return guarded([&] { m->m->head_gpu(h, batch, seq, logits, S(stream)); });
+}
+
+int lfm_model_verify(lfm_model *m, const int *ids, int batch, int seq, int n_draft,
+                     const float *draft, const float *u_accept, const float *u_sample,
+                     const int *n_valid, float temperature, float *probs, int *accepted,
+                     int *tokens, moe_stream_t stream) {
+  if (!m || batch < 0 || seq < 0) return MOE_ERR_INVALID_ARG;
+  if (batch > 0 && seq > 0 &&
+      (!ids || !u_sample || !probs || !accepted || !tokens || (n_draft > 0 && (!draft || !u_accept))))
+    return MOE_ERR_INVALID_ARG;
+  return guarded([&] {
+    m->m->verify_gpu(ids, batch, seq, n_draft, draft, u_accept, u_sample, n_valid, temperature, probs,
+                     accepted, tokens, S(stream));
+  });
 }
 
 int lfm_model_moe(lfm_model *m, int layer, moe_ctx **out) {

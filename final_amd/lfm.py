@@ -150,11 +150,14 @@ def verify_draft_workspace(batch, vocab) -> int:
 
 
 def verify_draft(target, draft, draft_ids, u_accept, u_sample, accepted, tokens, batch, n_draft,
-                 vocab, n_valid=None, workspace=None, workspace_bytes=0, stream=None):
-    _ck(_native.lib().lfm_verify_draft(_ptr(target), _ptr(draft), _ptr(draft_ids), _ptr(u_accept),
-                                       _ptr(u_sample), _ptr(n_valid), batch, n_draft, vocab,
-                                       _ptr(accepted), _ptr(tokens), _ptr(workspace),
-                                       workspace_bytes, _stream(stream)), "lfm_verify_draft")
+                 vocab, n_valid=None, ids_stride=None, workspace=None, workspace_bytes=0,
+                 stream=None):
+    _ck(_native.lib().lfm_verify_draft(_ptr(target), _ptr(draft), _ptr(draft_ids),
+                                       n_draft if ids_stride is None else ids_stride,
+                                       _ptr(u_accept), _ptr(u_sample), _ptr(n_valid), batch,
+                                       n_draft, vocab, _ptr(accepted), _ptr(tokens),
+                                       _ptr(workspace), workspace_bytes, _stream(stream)),
+        "lfm_verify_draft")
 
 
 def rope_tables(max_pos, head_dim=HEAD_DIM, theta=ROPE_THETA):
@@ -302,6 +305,14 @@ class LFM2Model:
     def head(self, h, batch, seq, logits, stream=None):
         _ck(_native.lib().lfm_model_head(self._m, _ptr(h), batch, seq, _ptr(logits),
                                          _stream(stream)), "lfm_model_head")
+
+    def verify(self, ids, batch, seq, n_draft, draft, u_accept, u_sample, probs, accepted, tokens,
+               temperature=1.0, n_valid=None, stream=None):
+        """Forward of ids [batch][seq] that end in n_draft drafts, and their verification."""
+        _ck(_native.lib().lfm_model_verify(self._m, _ptr(ids), batch, seq, n_draft, _ptr(draft),
+                                           _ptr(u_accept), _ptr(u_sample), _ptr(n_valid),
+                                           temperature, _ptr(probs), _ptr(accepted), _ptr(tokens),
+                                           _stream(stream)), "lfm_model_verify")
 
     def last_routing(self, layer: int, num_tokens: int) -> np.ndarray:
         """idx [T][4] of the MoE layer's last forward (valid until the next

@@ -203,8 +203,8 @@ int lfm_softmax_workspace(int rows, int dim, size_t *bytes);
 
 /* Verification of drafted tokens.  target [batch][n_draft + 1][vocab] holds the
  * target's probabilities after each draft (row 0: before the first), draft
- * [batch][n_draft][vocab] those that draft_ids [batch][n_draft] were drawn from,
- * u_accept [batch][n_draft] and u_sample [batch] random numbers of [0, 1);
+ * [batch][n_draft][vocab] those that draft_ids (sequence b's at draft_ids + b *
+ * ids_stride, ids_stride >= n_draft) were drawn from, u_accept [batch][n_draft] and u_sample [batch] random numbers of [0, 1);
  * n_valid [batch] how many drafts a sequence has (NULL: n_draft for all; held
  * to [0, n_draft]).  Draft i is accepted if all before it were and
  * u_accept * draft[i][id] < target[i][id].  Then one more token is drawn: after
@@ -219,7 +219,7 @@ int lfm_softmax_workspace(int rows, int dim, size_t *bytes);
  * (draft, draft_ids and u_accept may then be NULL).  n_draft at most 1024.
  * workspace: lfm_verify_draft_workspace bytes, as for lfm_kv_attention. */
 int lfm_verify_draft(const float *target, const float *draft, const int *draft_ids,
-                     const float *u_accept, const float *u_sample, const int *n_valid, int batch,
+                     long long ids_stride, const float *u_accept, const float *u_sample, const int *n_valid, int batch,
                      int n_draft, int vocab, int *accepted, int *tokens, void *workspace,
                      size_t workspace_bytes, moe_stream_t stream);
 int lfm_verify_draft_workspace(int batch, int vocab, size_t *bytes);
@@ -289,6 +289,16 @@ int lfm_model_layer_forward(lfm_model *m, int layer, float *h, int batch, int se
                             moe_stream_t stream);
 int lfm_model_head(lfm_model *m, const float *h, int batch, int seq, float *logits,
                    moe_stream_t stream);
+/* Forward of ids [batch][seq] (device int32) whose last n_draft tokens are drafts
+ * (0 <= n_draft < seq), then verification: probs [batch][n_draft + 1][vocab] gets
+ * the softmax (lfm_softmax with `temperature`) of the logits from the position
+ * before the first draft on, and accepted [batch] and tokens [batch][n_draft + 1]
+ * what lfm_verify_draft says of them; draft, u_accept, u_sample and n_valid are its
+ * arguments.  n_draft = 0 draws each sequence's next token. */
+int lfm_model_verify(lfm_model *m, const int *ids, int batch, int seq, int n_draft,
+                     const float *draft, const float *u_accept, const float *u_sample,
+                     const int *n_valid, float temperature, float *probs, int *accepted,
+                     int *tokens, moe_stream_t stream);
 /* The MoE context of a layer (NULL for a dense layer): moe_last_routing on it
  * reads that layer's routing until the next MoE layer runs (all layers share
  * one scratch). */

@@ -63,6 +63,13 @@ public:
   void embed_gpu(const int *ids, int batch, int seq_len, float *h, hipStream_t stream);
   void layer_forward_gpu(int layer, float *h, int batch, int seq_len, hipStream_t stream);
   void head_gpu(const float *h, int batch, int seq_len, float *logits, hipStream_t stream);
+  // Forward of ids [batch][seq] whose last n_draft tokens are drafts, the
+  // probabilities of the n_draft + 1 positions from the one before the first
+  // draft on into probs [batch][n_draft + 1][vocab], and their verification
+  // (lfm_verify_draft, whose arguments the others are).  0 <= n_draft < seq_len.
+  void verify_gpu(const int *ids, int batch, int seq_len, int n_draft, const float *draft,
+                  const float *u_accept, const float *u_sample, const int *n_valid,
+                  float temperature, float *probs, int *accepted, int *tokens, hipStream_t stream);
 
   int num_layers() const { return (int)layers_.size(); }
   int max_tokens() const { return max_batch_ * max_seq_; }

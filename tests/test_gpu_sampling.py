@@ -183,6 +183,75 @@ def test_verify_borders(V):
 
 
 @pytest.mark.gpu
+def test_verify_of_strided_ids():
+    from final_amd import hip, lfm
+    r = np.random.default_rng(8)
+    B, K, V = 5, 3, 900
+    t, d = probs(r, B, K + 1, V), probs(r, B, K, V)
+    rows = r.integers(0, V, (B, 11)).astype(np.int32)
+    ua, us = 0.01 * r.random((B, K), dtype=np.float32), r.random(B, dtype=np.float32)
+    ids = dev(rows)
+    acc, tok = hip.DeviceArray((B,), np.int32), hip.DeviceArray((B, K + 1), np.int32)
+    need = lfm.verify_draft_workspace(B, V)
+    ws = hip.DeviceArray((need,), np.uint8)
+    lfm.verify_draft(dev(t), dev(d), ids.ptr + 4 * 8, dev(ua), dev(us), acc, tok, B, K, V, ids_stride=11, workspace=ws,
+                     workspace_bytes=need)
+    want = R.verify(t, d, rows[:, 8:], ua, us, np.full(B, K))
+    assert want[0].max() > 0
+    same((acc.download(), tok.download()), want)
+
+
+@pytest.mark.gpu
+def test_model_verify():
+    """The model's path: its probabilities are the softmax of the logits its head gives at each position,
+    and its tokens what verification of them gives; n_draft = 0 draws the next token."""
+    from final_amd import _native, hip, lfm
+    r = np.random.default_rng(6)
+    B, S, K, V, H, temp = 3, 20, 4, lfm.VOCAB, lfm.HIDDEN, 0.8
+    model = lfm.LFM2Model(num_layers=2, layer_types=[1, 0], num_dense_layers=1, max_batch=4, max_seq=32, seed=5)
+    ids = r.integers(0, V, (B, S)).astype(np.int32)
+    dids = dev(ids)
+    d = probs(r, B, K, V)
+    d[0] = np.float32(1e-9)  # its drafts are accepted
+    ua, us = r.random((B, K), dtype=np.float32), r.random(B, dtype=np.float32)
+    n = np.array([K, K, 2], np.int32)
+    pt, acc, tok = hip.DeviceArray((B, K + 1, V)), hip.DeviceArray((B,), np.int32), hip.DeviceArray((B, K + 1), np.int32)
+    model.verify(dids, B, S, K, dev(d), dev(ua), dev(us), pt, acc, tok, temperature=temp, n_valid=dev(n))
+    p = pt.download()
+    same((acc.download(), tok.download()), R.verify(p, d, ids[:, S - K:], ua, us, n))
+    assert acc.download()[0] == K
+    # the head of shortened sequences of the same hidden states
+    h = hip.DeviceArray((B * S, H))
+    model.embed(dids, B, S, h)
+    for layer in range(2):
+        model.layer_forward(layer, h, B, S)
+    hs = h.download().reshape(B, S, H)
+    logits = hip.DeviceArray((B, V))
+    for i in range(K + 1):
+        m = S - K + i
+        model.head(dev(hs[:, :m]), B, m, logits)
+        x = logits.download()
+        # the head's products of 2048 values round in another order there: 2048 + 6 steps of 2^-24 of the sum
+        # of their magnitudes, which sqrt(2048) |h| |w| bounds; |h| is the norm's sqrt(2048), |w| below 1.1
+        w = np.exp((2 * 2054 * EPS * np.sqrt(2048) * 1.1) / temp) - 1
+        ref = R.softmax(x, temp)
+        assert np.abs(p[:, i] - ref).max() <= (2 * w + 1e-5) * ref.max()
+    assert model.status() == 0
+    t0 = hip.DeviceArray((B, 1), np.int32)
+    p0 = hip.DeviceArray((B, 1, V))
+    model.verify(dids, B, S, 0, None, None, dev(us), p0, acc, t0, temperature=temp)
+    same((acc.download(), t0.download()), R.verify(p0.download(), None, None, None, us, np.zeros(B)))
+    for args in ((B, S, S), (B, S, -1), (5, S, K), (B, 33, K)):
+        with pytest.raises(_native.MoeError) as e:
+            model.verify(dids, *args, dev(d), dev(ua), dev(us), pt, acc, tok)
+        assert e.value.status == _native.MOE_ERR_INVALID_ARG
+    with pytest.raises(_native.MoeError) as e:
+        model.verify(dids, B, S, K, dev(d), dev(ua), dev(us), pt, acc, tok, temperature=0.0)
+    assert e.value.status == _native.MOE_ERR_INVALID_ARG
+    model.close()
+
+
+@pytest.mark.gpu
 def test_verify_of_many_random_numbers():
     """One distribution at many random numbers: every id is drawn at its place of the running sum."""
     r = np.random.default_rng(0)

@@ -101,21 +101,21 @@ def test_softmax_and_verify_refused(lib):
         assert soft(**kw) == inv, kw
     assert soft(rows=0, x=None, y=None) == 0
 
-    def ver(target=A, draft=A, ids=A, ua=A, us=A, b=2, k=3, v=10, acc=A, tok=A, ws=A, n=1 << 40):
-        return L.lfm_verify_draft(target, draft, ids, ua, us, None, b, k, v, acc, tok, ws, n, None)
+    def ver(target=A, draft=A, ids=A, stride=3, ua=A, us=A, b=2, k=3, v=10, acc=A, tok=A, ws=A, n=1 << 40):
+        return L.lfm_verify_draft(target, draft, ids, stride, ua, us, None, b, k, v, acc, tok, ws, n, None)
 
     for kw in (dict(target=None), dict(draft=None), dict(ids=None), dict(ua=None), dict(us=None), dict(acc=None),
-               dict(tok=None), dict(b=-1), dict(k=-1), dict(v=0)):
+               dict(tok=None), dict(b=-1), dict(k=-1), dict(v=0), dict(stride=2), dict(ws=None), dict(n=1), dict(ws=A + 8)):
         assert ver(**kw) == inv, kw
     assert ver(k=1025) == ver(b=65536) == lib.MOE_ERR_UNSUPPORTED
     assert ver(b=0, target=None) == 0
+    assert L.lfm_model_verify(None, A, 1, 4, 1, A, A, A, None, 1.0, A, A, A, None) == inv
     n = ctypes.c_size_t(0)
     assert L.lfm_softmax_workspace(-1, 4, ctypes.byref(n)) == L.lfm_softmax_workspace(1, 0, ctypes.byref(n)) == inv
     assert L.lfm_verify_draft_workspace(-1, 4, ctypes.byref(n)) == inv
-    assert L.lfm_softmax_workspace(1, 65536, ctypes.byref(n)) == 0
-    if n.value:
-        assert soft(rows=1, dim=65536, xs=65536, ys=65536, ws=None) == inv
-        assert soft(rows=1, dim=65536, xs=65536, ys=65536, n=n.value - 1) == inv
+    assert L.lfm_softmax_workspace(1, 70000, ctypes.byref(n)) == 0 and n.value > 0
+    assert soft(rows=1, dim=70000, xs=70000, ys=70000, ws=None) == inv
+    assert soft(rows=1, dim=70000, xs=70000, ys=70000, n=n.value - 1) == inv
 
 
 def test_plain_forms():
