@@ -293,7 +293,10 @@ CASES = [  # heads, kv, page, new, own, prefix
     (32, 8, 16, [1, 1, 1], [7, 150, 16], 129), (32, 8, 64, [5, 3, 0, 8], [5, 200, 9, 64], 33),
     (8, 8, 16, [1, 2], [40, 1000], 0), (16, 2, 32, [4, 1], [100, 2], 64), (64, 1, 16, [2], [77], 48),
     (6, 3, 128, [33], [33], 0), (32, 8, 128, [100, 37], [300, 37], 500), (5, 5, 16, [17, 16], [17, 90], 15),
-    (32, 8, 16, [1] * 70, list(range(1, 71)), 40), (12, 1, 16, [1], [4000], 0)]
+    (32, 8, 16, [1] * 70, list(range(1, 71)), 40), (12, 1, 16, [1], [4000], 0),
+    # one to four column tiles of own positions, alone, beside a prefix of one column tile and of several
+    (32, 8, 16, [3], [100], 70), (32, 8, 32, [3, 2], [100, 600], 300), (32, 8, 16, [6, 2], [9, 700], 0),
+    (32, 8, 16, [4], [600], 0), (16, 8, 64, [1, 2, 1], [600, 2, 31], 1500), (64, 8, 16, [2], [40], 2100)]
 
 
 @pytest.mark.gpu
@@ -310,6 +313,77 @@ def test_attention(fmt, heads, kv, page, new, own, prefix):
     got = attend(pool, q, x, heads, flag=flag)
     assert np.isfinite(got).all() and flag.download()[0] == 0
     check(pool, q, x, heads, got)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", [R.BF16, R.FP8])
+@pytest.mark.parametrize("heads,kv,page,new,own,prefix,max_len", [
+    (4, 1, 16, [1], [9000], 0, 1),            # one part: more than 32 tiles a wave
+    (4, 1, 32, [1, 1], [9000, 40], 0, 1 << 20),  # a hint far above the lengths
+    (32, 8, 64, [512], [512], 4200, 512)])    # and of the prefix
+def test_attention_of_many_tiles_a_wave(fmt, heads, kv, page, new, own, prefix, max_len):
+    say(f"[kv attention] fmt={fmt} heads={heads}/{kv} new={new} own={own} prefix={prefix} hint={max_len}")
+    r = np.random.default_rng(fmt)
+    pool = Pool(fmt, kv, page, len(new) * -(-max(own) // page) + -(-prefix // page) + 2)
+    q = Seqs(r, pool, new, own, prefix=prefix, max_len=max_len)
+    fill(r, pool, q)
+    x = draws(r, (q.tokens, heads * 64), sizes=False)
+    got = attend(pool, q, x, heads)
+    check(pool, q, x, heads, got)
+    assert np.array_equal(bits(attend(pool, q, x, heads)), bits(got))  # and the same bits again
+
+
+@pytest.mark.gpu
+def test_output_rows_of_their_own_length():
+    from final_amd import hip, lfm
+    r = np.random.default_rng(4)
+    pool = Pool(R.INT8, 8, 16, 60)
+    q = Seqs(r, pool, [2, 1], [300, 35], prefix=100)
+    fill(r, pool, q)
+    x = draws(r, (q.tokens, 2048), sizes=False)
+    want = attend(pool, q, x, 32)
+    wide = np.zeros((q.tokens, 2048 + 12), np.float32)
+    wide[:, 8:8 + 2048] = x
+    dx, do = dev(wide), dev(np.full((q.tokens, 2052), 7.0, np.float32))
+    need = lfm.kv_attention_workspace(pool.c, q.c)
+    ws = hip.DeviceArray((max(need, 16),), np.uint8)
+    lfm.kv_attention(pool.c, q.c, dx.ptr + 32, 2060, do, ld_out=2052, workspace=ws, workspace_bytes=need)
+    got = do.download()
+    assert np.array_equal(bits(got[:, :2048]), bits(want)) and (got[:, 2048:] == 7.0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", [R.INT8, R.F32])
+def test_pages_beyond_4_gib(fmt):
+    """The same sequence in a pool's first and last pages, whose addresses are 4.5 GB and more apart."""
+    from final_amd import hip, lfm
+    r = np.random.default_rng(fmt)
+    size = np.dtype(R.DTYPE[fmt]).itemsize
+    page_bytes = 8 * 4096 * 64 * size
+    pages = (9 << 29) // page_bytes
+    k, v = (hip.DeviceArray((pages * page_bytes,), np.uint8) for _ in range(2))
+    scaled = fmt == R.INT8
+    ks, vs = ((hip.DeviceArray((pages * 8 * 4096,)) for _ in range(2)) if scaled else (None, None))
+    cache = lfm.KVCache(fmt, pages, 4096, k, v, ks, vs)
+    n = 5000
+    x = dev(draws(r, (n, lfm.QKV_COLS), sizes=False))
+    own, got = dev(np.array([n], np.int32)), []
+    for table in ([0, 1], [pages - 1, pages - 2]):
+        t = dev(np.array([table], np.int32))
+        b = lfm.KVBatch(1, own, t, 2, max_new=n, max_len=n)
+        flag = dev(np.zeros(1, np.int32))
+        lfm.kv_write(cache, b, x, lfm.QKV_COLS, bad_flag=flag)
+        out = [hip.DeviceArray((n, 512)) for _ in range(2)]
+        lfm.kv_read(cache, b, out[0], out[1], n, bad_flag=flag)
+        one = lfm.KVBatch(1, own, t, 2, max_new=1, max_len=n)
+        need = lfm.kv_attention_workspace(cache, one)
+        ws, o = hip.DeviceArray((max(need, 16),), np.uint8), hip.DeviceArray((1, 2048))
+        lfm.kv_attention(cache, one, x, lfm.QKV_COLS, o, workspace=ws, workspace_bytes=need, bad_flag=flag)
+        got.append([a.download() for a in out + [o]])
+        assert flag.download()[0] == 0
+    assert all(np.array_equal(bits(a), bits(b)) for a, b in zip(*got))
+    if fmt == R.F32:
+        assert np.array_equal(bits(got[0][0]), bits(x.download()[:, 2048:2560]))
 
 
 @pytest.mark.gpu
