@@ -16,10 +16,16 @@ namespace lfm {
 // ---------------------------------------------------------------------------
 
 // 16 lanes take a row of 64 (a token's q, k or v head), four floats each, R rows
-// one after the other; block (x, sequence).  Every load that hangs on nothing but
-// the sequence stands in front, without a branch: pages, then rows.
+// one after the other; block (x, sequence).  A row's largest magnitude is found
+// over its 16 lanes by DPP moves, so nothing goes through LDS and no block waits.
+// What bounds them is memory: every load that hangs on nothing but the sequence
+// stands in front, without a branch, pages and then R rows, so that four rows a
+// lane are in flight.  64 ragged sequences of up to 512 tokens and 8 heads in fp8 (117
+// MB): written in 33 us (3.5 TB/s, three quarters of it reads), read back in 23 us
+// (5.1 TB/s); 20011 bf16 tokens (123 MB) are read in 26 us.  A single token takes 2.4
+// and 37 take 3.1 us: a launch, and the table, page and row one after the other.
 
-// The page of own position pos of sequence b; -1 (and the flag) outside the cache.
+// The page, or -1 (and the flag) where it is outside the cache.
 __device__ __forceinline__ int kv_page(const KvArgs &a, int page) {
   if (page >= 0 && page < a.num_pages) return page;
   kv_flag(a.bad);
@@ -131,8 +137,9 @@ __global__ __launch_bounds__(256) void kv_read_kernel(KvArgs a, float *k_out, fl
 // loads 16 bytes of key c of each half tile, which is its operand of S^T up to a
 // permutation of the dimensions (the same in q's), and four values, dimensions 4c
 // .. 4c+3, of the keys 4g + i, whose weights S^T leaves in this lane: block db of
-// O^T takes dimension 4c + db from each.  The four waves of a block take every
-// fourth tile and join their sums through LDS at the end.
+// O^T takes dimension 4c + db from each.  The tiles are dealt to the waves of a
+// part's blocks in turn, which join their sums through LDS at the end; a part that
+// is not the only one leaves them in the workspace to kv_join_kernel.
 //
 // The running maximum is only raised when a score passes it by kRaise: weights
 // then reach 2^kRaise, and most tiles need no exchange between lanes and no
@@ -424,11 +431,6 @@ __device__ __forceinline__ void flash_part(const KvArgs &a, const FlashArgs &f, 
     }
   }
 
-  auto in_cache = [&](int page) {
-    if (page >= 0 && page < a.num_pages) return page;
-    kv_flag(a.bad);
-    return -1;
-  };
   auto load = [&](int t, int page0, int page1, Raw &r) {
 #pragma unroll
     for (int hb = 0; hb < 2; ++hb) {
@@ -650,10 +652,10 @@ __device__ __forceinline__ void flash_part(const KvArgs &a, const FlashArgs &f, 
   Raw ra, rb;  // two tiles: one computed, one on its way
   int pages = 0;
   if (t0 < t_end) {
-    pages = in_cache(page_of(t0));
+    pages = kv_page(a, page_of(t0));
     const int half0 = __builtin_amdgcn_readlane(first_pages, 0);
     const int half1 = t0 * kKeys + 16 < len ? __builtin_amdgcn_readlane(first_pages, 1) : half0;
-    load(t0, in_cache(half0), in_cache(half1), ra);
+    load(t0, kv_page(a, half0), kv_page(a, half1), ra);
   }
   // q's parts, scaled so that a score is the log2 of its weight
 #pragma unroll
@@ -677,7 +679,7 @@ __device__ __forceinline__ void flash_part(const KvArgs &a, const FlashArgs &f, 
   auto step = [&](Raw &r, Raw &rn) {
     const bool more = t + stride < t_end;
     const int next = more ? t + stride : t, i = (n + (more ? 1 : 0)) & 31;
-    if (more && i == 0) pages = in_cache(page_of(next));
+    if (more && i == 0) pages = kv_page(a, page_of(next));
     tile(t, r, rn, next, __builtin_amdgcn_readlane(pages, 2 * i), __builtin_amdgcn_readlane(pages, 2 * i + 1));
     t += stride;
     ++n;
@@ -738,6 +740,18 @@ __device__ __forceinline__ void flash_part(const KvArgs &a, const FlashArgs &f, 
   }
 }
 
+// What bounds it, by the columns (8 kv heads, 4 heads each):
+// - one token a sequence: the cache's bytes.  64 ragged sequences of up to 2048 int8
+//   positions (88 MB) take 22 us, 4.0 TB/s with the start of the launch and of the
+//   loads, 4 of 65536 bf16 positions (537 MB) 93 us, 5.8 TB/s: two tiles a wave are
+//   on their way with no branch between their loads.
+// - 4 column tiles (a prefix of 64 sequences, or a prompt): the exponentials, the
+//   splits of weights and the matrix instructions, which keep a SIMD's vector unit
+//   from issuing for half of their 16 cycles.  8192 fp8 positions for 64 x 1 token:
+//   11.5 us of 22; the rest is the launch, the first loads, the join of the waves and
+//   the own positions beside.
+// - short caches: a chain of loads (length, page, rows), 10 us for 300 positions.
+
 // Waves a SIMD holds, by the registers a tile's columns take.
 constexpr int flash_waves(int fmt, int ct) { return fmt == LFM_KV_F32 ? 2 : ct == 0 ? 4 : ct == 1 ? 3 : 2; }
 
@@ -775,7 +789,9 @@ void kv_prefix_flash_kernel(KvArgs a, FlashArgs f, int prefix_blocks, int own_gr
 }
 
 // Joins the parts of a token's head, a wave per row: 16 lanes take a part's 64
-// sums, so four parts are loaded at a time, and a lane a part's maximum.
+// sums, so four parts are loaded at a time, and a lane a part's maximum.  Latency
+// bounds it: 64 x 32 rows of 9 parts 4.2 us, 4 x 32 rows of 16 parts 5.0 us, half of
+// it the launch.
 __global__ __launch_bounds__(256) void kv_join_kernel(KvArgs a, FlashArgs f) {
   KvSeq s;
   if (!kv_seq<true>(a, blockIdx.y, s)) return;
