@@ -222,7 +222,9 @@ hipError_t launch_softmax(const float *x, long long xs, float *y, long long ys, 
                           float temperature, void *ws, hipStream_t st) {
   const float c = (float)(1.4426950408889634 / (double)temperature);
   const int whole = whole_rows(rows, dim), left = rows - whole;
-  if (whole > 0) softmax_rows_launch(x, xs, y, ys, whole, 1, dim, c, st);
+  constexpr int kMostRows = 1 << 21;  // of a launch: its threads are counted in 32 bits
+  for (long long r0 = 0; r0 < whole; r0 += kMostRows)
+    softmax_rows_launch(x + r0 * xs, xs, y + r0 * ys, ys, (int)std::min<long long>(whole - r0, kMostRows), 1, dim, c, st);
   x += whole * xs;
   y += whole * ys;
   if (left > 0 && x != y && share_rows(left, whole, dim)) {

@@ -61,6 +61,14 @@ def test_softmax(rows, dim, t):
 
 
 @pytest.mark.gpu
+def test_softmax_of_more_rows_than_a_launch():
+    rows, dim = (1 << 22) + 3, 2
+    say(f"[softmax] rows={rows} dim={dim}")
+    x = 3 * np.random.default_rng(22).standard_normal((rows, dim), dtype=np.float32)
+    close(run_softmax(dev(x), dev(np.zeros_like(x)), rows, dim, 1.0), x, 1.0)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("rows,dim", [(4, 700), (4, 65536), (300, 9001)])
 def test_softmax_of_masks_and_extremes(rows, dim):
     r = np.random.default_rng(dim)
