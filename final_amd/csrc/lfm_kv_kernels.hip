@@ -973,7 +973,9 @@ hipError_t launch_kv_attention(const KvArgs &a, const float *q, int ld, float *o
                     ld, ldo, heads, heads / a.kv_heads, p.own_parts, p.prefix_parts, rows};
   const long long own_blocks = (long long)a.kv_heads * p.own_parts * p.own_groups * a.batch;
   const long long prefix_blocks = (long long)a.kv_heads * p.prefix_parts * p.prefix_groups;
-  if (p.own_groups > 65535 || own_blocks + prefix_blocks > 0x7FFFFFFF) return hipErrorInvalidValue;
+  // beside a prefix all blocks are in x, whose threads are counted in 32 bits
+  if (p.own_groups > 65535 || own_blocks + prefix_blocks > (p.prefix_parts ? 0xFFFFFF : 0x7FFFFFFF))
+    return hipErrorInvalidValue;
   return by_format(a.format, [&](auto fmt) -> hipError_t {
     constexpr int FMT = fmt(), MOST = FMT == LFM_KV_F32 ? 2 : 4;
     hipError_t e = by_columns<MOST>(p.own_ct, [&](auto own) -> hipError_t {

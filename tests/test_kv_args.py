@@ -84,6 +84,9 @@ def test_arguments_refused(lib):
     if n.value:
         assert attend(lib, c, big, ws=None) == inv and attend(lib, c, big, n=n.value - 1) == inv
         assert attend(lib, c, big, ws=A + 8) == inv
+    # 2^24 blocks of 256 threads beside a prefix
+    many = batch(lib, batch=65535, tokens=65535, max_new=1, prefix_len=16, prefix_pages=A)
+    assert attend(lib, cache(lib, kv_heads=256), many, heads=256, ld=256 * 64, ldo=256 * 64, n=1 << 50) == uns
     # nothing to do
     for kw in (dict(batch=0, tokens=0), dict(max_new=0, tokens=0)):
         assert write(lib, c, batch(lib, **kw), qkv=None) == 0 and attend(lib, c, batch(lib, **kw), q=None) == 0
