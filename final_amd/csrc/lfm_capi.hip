@@ -233,9 +233,9 @@ int lfm_verify_draft_workspace(int batch, int vocab, size_t *bytes) {
 }
 
 int lfm_verify_draft(const float *target, const float *draft, const int *draft_ids,
-                     long long ids_stride, const float *u_accept, const float *u_sample, const int *n_valid, int batch,
-                     int n_draft, int vocab, int *accepted, int *tokens, void *workspace,
-                     size_t workspace_bytes, moe_stream_t stream) {
+                     long long ids_stride, const float *u_accept, const float *u_sample,
+                     const int *n_valid, int batch, int n_draft, int vocab, int *accepted,
+                     int *tokens, void *workspace, size_t workspace_bytes, moe_stream_t stream) {
   if (batch < 0 || n_draft < 0 || vocab <= 0) return MOE_ERR_INVALID_ARG;
   if (batch == 0) return MOE_OK;
   if (batch > 65535 || n_draft > 1024) return MOE_ERR_UNSUPPORTED;

@@ -153,7 +153,7 @@ void LFM2Model::verify_gpu(const int *ids, int batch, int seq_len, int n_draft, 
                            float temperature, float *probs, int *accepted, int *tokens,
                            hipStream_t stream) {
   check_shape(batch, seq_len);
-  if (n_draft < 0 || (seq_len > 0 && n_draft >= seq_len))
+  if (n_draft < 0 || n_draft > 1024 || (seq_len > 0 && n_draft >= seq_len))
     throw std::invalid_argument("LFM2Model::verify: n_draft");
   if (!(temperature >= 0x1p-120f && temperature <= 0x1p120f))
     throw std::invalid_argument("LFM2Model::verify: temperature");

@@ -154,8 +154,9 @@ typedef struct lfm_kv_batch {
  * only then) q and k are first normalised and rotated as lfm_qk_norm_rope does,
  * bit for bit, for position prefix_len + own position: q in place in columns
  * [0, heads*64), k on its way to the cache (qkv keeps its own).  A position of
- * max_pos, the tables' rows, or more sets *bad_flag and leaves the token out.  qkv 16-byte aligned, ld, k_col and v_col multiples of 4,
- * heads*64 <= k_col, k_col + kv_heads*64 <= v_col. */
+ * max_pos, the tables' rows, or more sets *bad_flag and leaves the token out.
+ * qkv 16-byte aligned, ld, k_col and v_col multiples of 4, heads*64 <= k_col,
+ * k_col + kv_heads*64 <= v_col. */
 int lfm_kv_write(const lfm_kv_cache *cache, const lfm_kv_batch *batch, float *qkv, int ld,
                  int heads, int k_col, int v_col, const float *q_weight, const float *k_weight,
                  const float *cos_table, const float *sin_table, int max_pos, int *bad_flag,
@@ -174,9 +175,9 @@ int lfm_kv_read(const lfm_kv_cache *cache, const lfm_kv_batch *batch, float *k_o
  * attention of lfm_attention for new tokens whose keys and values, their own
  * included, are in the cache.  q is read from columns [0, heads*64) of qkv
  * [tokens][ld], out has rows of ld_out.  heads a multiple of kv_heads, at most
- * 64 of them for each.  A token that sees no position (its pages are outside the
- * cache) gets zeros.  The prefix's
- * keys and values are read once for all sequences.  Sums, maxima and weights
+ * 64 of them for each.  out does not overlap the columns that q is read from.  A
+ * token that sees no position (its pages are outside the cache) gets zeros.  The
+ * prefix's keys and values are read once for all sequences.  Sums, maxima and weights
  * are fp32.  A key that is not finite makes the outputs of the tokens that see
  * it, for its heads, NaN, and a value that is not finite those of its column
  * not finite; what a token does not see does not reach it.
@@ -204,14 +205,15 @@ int lfm_softmax_workspace(int rows, int dim, size_t *bytes);
 /* Verification of drafted tokens.  target [batch][n_draft + 1][vocab] holds the
  * target's probabilities after each draft (row 0: before the first), draft
  * [batch][n_draft][vocab] those that draft_ids (sequence b's at draft_ids + b *
- * ids_stride, ids_stride >= n_draft) were drawn from, u_accept [batch][n_draft] and u_sample [batch] random numbers of [0, 1);
- * n_valid [batch] how many drafts a sequence has (NULL: n_draft for all; held
- * to [0, n_draft]).  Draft i is accepted if all before it were and
- * u_accept * draft[i][id] < target[i][id].  Then one more token is drawn: after
- * a rejected draft i from max(target[i] - draft[i], 0), or from target[i] where
- * that has no positive sum; after n_valid accepted drafts from target[n_valid].
- * It is the lowest id up to which the weights' sum exceeds u_sample times their
- * whole sum, in 64 bits; -1 where no weight is positive.  Weights that are NaN
+ * ids_stride, ids_stride >= n_draft) were drawn from, u_accept [batch][n_draft]
+ * and u_sample [batch] random numbers of [0, 1); n_valid [batch] how many drafts
+ * a sequence has (NULL: n_draft for all; held to [0, n_draft]).  Draft i is
+ * accepted if all before it were and u_accept * draft[i][id] < target[i][id].
+ * Then one more token is drawn: after a rejected draft i from max(target[i] -
+ * draft[i], 0), or from target[i] where that has no positive sum; after n_valid
+ * accepted drafts from target[n_valid].  It is the lowest id up to which the
+ * weights' sum exceeds u_sample times their whole sum, in 64 bits; -1 where no
+ * weight is positive.  Weights that are NaN
  * or below 0 count as 0 (an infinite one leaves -1), and an id outside [0, vocab)
  * is rejected.
  * accepted [batch] = the number of accepted drafts; tokens [batch][n_draft + 1]
@@ -219,9 +221,9 @@ int lfm_softmax_workspace(int rows, int dim, size_t *bytes);
  * (draft, draft_ids and u_accept may then be NULL).  n_draft at most 1024.
  * workspace: lfm_verify_draft_workspace bytes, as for lfm_kv_attention. */
 int lfm_verify_draft(const float *target, const float *draft, const int *draft_ids,
-                     long long ids_stride, const float *u_accept, const float *u_sample, const int *n_valid, int batch,
-                     int n_draft, int vocab, int *accepted, int *tokens, void *workspace,
-                     size_t workspace_bytes, moe_stream_t stream);
+                     long long ids_stride, const float *u_accept, const float *u_sample,
+                     const int *n_valid, int batch, int n_draft, int vocab, int *accepted,
+                     int *tokens, void *workspace, size_t workspace_bytes, moe_stream_t stream);
 int lfm_verify_draft_workspace(int batch, int vocab, size_t *bytes);
 
 /* Rotary tables [max_pos][head_dim] in host memory, computed as
@@ -290,7 +292,7 @@ int lfm_model_layer_forward(lfm_model *m, int layer, float *h, int batch, int se
 int lfm_model_head(lfm_model *m, const float *h, int batch, int seq, float *logits,
                    moe_stream_t stream);
 /* Forward of ids [batch][seq] (device int32) whose last n_draft tokens are drafts
- * (0 <= n_draft < seq), then verification: probs [batch][n_draft + 1][vocab] gets
+ * (0 <= n_draft < seq, at most 1024), then verification: probs [batch][n_draft + 1][vocab] gets
  * the softmax (lfm_softmax with `temperature`) of the logits from the position
  * before the first draft on, and accepted [batch] and tokens [batch][n_draft + 1]
  * what lfm_verify_draft says of them; draft, u_accept, u_sample and n_valid are its

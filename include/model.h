@@ -66,7 +66,8 @@ public:
   // Forward of ids [batch][seq] whose last n_draft tokens are drafts, the
   // probabilities of the n_draft + 1 positions from the one before the first
   // draft on into probs [batch][n_draft + 1][vocab], and their verification
-  // (lfm_verify_draft, whose arguments the others are).  0 <= n_draft < seq_len.
+  // (lfm_verify_draft, whose arguments the others are).  0 <= n_draft < seq_len,
+  // n_draft at most 1024.
   void verify_gpu(const int *ids, int batch, int seq_len, int n_draft, const float *draft,
                   const float *u_accept, const float *u_sample, const int *n_valid,
                   float temperature, float *probs, int *accepted, int *tokens, hipStream_t stream);

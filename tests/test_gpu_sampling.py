@@ -260,6 +260,16 @@ def test_model_verify():
 
 
 @pytest.mark.gpu
+def test_model_verify_refuses_more_drafts_than_verification_takes():
+    from final_amd import _native, hip, lfm
+    model = lfm.LFM2Model(num_layers=1, layer_types=[1], num_dense_layers=1, max_batch=1, max_seq=1026, seed=5)
+    x = hip.DeviceArray((16,))  # refused before anything reads it
+    with pytest.raises(_native.MoeError) as e:
+        model.verify(x, 1, 1026, 1025, x, x, x, x, x, x)
+    assert e.value.status == _native.MOE_ERR_INVALID_ARG
+
+
+@pytest.mark.gpu
 def test_verify_of_many_random_numbers():
     """One distribution at many random numbers: every id is drawn at its place of the running sum."""
     r = np.random.default_rng(0)
