@@ -2,6 +2,7 @@
 // (lfm_model_*, include/lfm_capi.h).  Reference: src/model.cu:124-569.
 #include "model.h"
 
+#include <algorithm>
 #include <iostream>
 #include <new>
 #include <stdexcept>
@@ -164,13 +165,23 @@ void LFM2Model::verify_gpu(const int *ids, int batch, int seq_len, int n_draft, 
   // first buffer, the samplers' scratch (200 bytes a row) to its widest.
   const long long H = (long long)HIDDEN_SIZE;
   const int per = n_draft + 1, rows = batch * per;
-  for (int i = 0; i < per; ++i)
-    check(lfm_rmsnorm(hidden_ + (size_t)(seq_len - per + i) * H, (long long)seq_len * H,
-                      norm_->weight_gpu(), ws_->normed + i * H, (long long)per * H, batch, (int)H, stream),
-          "lfm_rmsnorm");
+  const float *first = hidden_ + (size_t)(seq_len - per) * H;
+  if (batch < per)  // a sequence's positions at a time, or a position of every sequence
+    for (int b = 0; b < batch; ++b)
+      check(lfm_rmsnorm(first + (size_t)b * seq_len * H, H, norm_->weight_gpu(), ws_->normed + (size_t)b * per * H, H,
+                        per, (int)H, stream),
+            "lfm_rmsnorm");
+  else
+    for (int i = 0; i < per; ++i)
+      check(lfm_rmsnorm(first + i * H, (long long)seq_len * H, norm_->weight_gpu(), ws_->normed + i * H,
+                        (long long)per * H, batch, (int)H, stream),
+            "lfm_rmsnorm");
   const float *head = lm_head_.size() ? lm_head_.gpu() : embed_tokens_.gpu();
-  check(lfm_gemm_nt(ws_->normed, head, probs, nullptr, rows, (int)vocab_, (int)H, stream),
-        "lfm_gemm_nt lm_head");
+  const int most = std::max(1, (1 << 28) / (int)std::max((long long)vocab_, H));  // rows of a product: 1 GiB of logits
+  for (int r0 = 0; r0 < rows; r0 += most)
+    check(lfm_gemm_nt(ws_->normed + (size_t)r0 * H, head, probs + (size_t)r0 * vocab_, nullptr,
+                      std::min(most, rows - r0), (int)vocab_, (int)H, stream),
+          "lfm_gemm_nt lm_head");
   const size_t scratch = (size_t)batch * seq_len * 3 * H * sizeof(float);
   check(lfm_softmax(probs, (long long)vocab_, probs, (long long)vocab_, rows, (int)vocab_, temperature,
                     ws_->proj, scratch, stream),

@@ -260,6 +260,37 @@ def test_model_verify():
 
 
 @pytest.mark.gpu
+def test_model_verify_of_many_positions():
+    """64 x 257 positions of 65536 logits are more than one product of the head takes: the last position's
+    probabilities of every sequence are those of its forward."""
+    import ctypes
+
+    from final_amd import hip, lfm
+    B, S, K, V, temp = 64, 260, 256, lfm.VOCAB, 1.0
+    r = np.random.default_rng(7)
+    model = lfm.LFM2Model(num_layers=1, layer_types=[1], num_dense_layers=1, max_batch=B, max_seq=S, seed=5)
+    ids = r.integers(0, V, (B, S)).astype(np.int32)
+    dids, logits = dev(ids), hip.DeviceArray((B, V))
+    model.forward(dids, B, S, logits)
+    ref = R.softmax(logits.download(), temp)
+    p, d = hip.DeviceArray((B, K + 1, V)), hip.DeviceArray((B, K, V))
+    d.fill_async(0)  # u * 0 < p: every draft is accepted
+    ua, us = dev(r.random((B, K), dtype=np.float32)), r.random(B, dtype=np.float32)
+    acc, tok = hip.DeviceArray((B,), np.int32), hip.DeviceArray((B, K + 1), np.int32)
+    model.verify(dids, B, S, K, d, ua, dev(us), p, acc, tok, temperature=temp)
+    assert (acc.download() == K).all()
+    got = tok.download()
+    assert np.array_equal(got[:, :K], ids[:, S - K:])
+    row = np.empty((1, V), np.float32)
+    w = np.exp((2 * 2054 * EPS * np.sqrt(2048) * 1.1) / temp) - 1  # as in test_model_verify
+    for b in range(B):
+        assert hip.rt().hipMemcpy(row.ctypes.data, p.ptr + 4 * ((b * (K + 1) + K) * V), row.nbytes, 2) == 0
+        assert np.abs(row[0] - ref[b]).max() <= (2 * w + 1e-5) * ref[b].max()
+        assert got[b, K] == R.verify(row[None], None, None, None, us[b:b + 1], np.zeros(1))[1][0, 0]
+    model.close()
+
+
+@pytest.mark.gpu
 def test_model_verify_refuses_more_drafts_than_verification_takes():
     from final_amd import _native, hip, lfm
     model = lfm.LFM2Model(num_layers=1, layer_types=[1], num_dense_layers=1, max_batch=1, max_seq=1026, seed=5)
@@ -267,6 +298,7 @@ def test_model_verify_refuses_more_drafts_than_verification_takes():
     with pytest.raises(_native.MoeError) as e:
         model.verify(x, 1, 1026, 1025, x, x, x, x, x, x)
     assert e.value.status == _native.MOE_ERR_INVALID_ARG
+    model.close()
 
 
 @pytest.mark.gpu
@@ -300,3 +332,82 @@ def test_logits_to_verified_tokens():
     assert (ids >= 0).all()
     ua = r.random((B, K), dtype=np.float32)
     same(run_verify(pt, pd, ids, ua, us), R.verify(pt, pd, ids, ua, us, np.full(B, K)))
+
+
+@pytest.mark.gpu
+def test_a_step_with_drafts_as_a_graph():
+    """Keys and values written, attention, a head, softmax and verification, captured once and replayed with
+    eager work between, as the sequences advance by what was accepted: each replay's bits are the eager ones."""
+    import ctypes
+
+    from final_amd import hip, lfm
+    r = np.random.default_rng(8)
+    B, K, V, page, per, prefix = 3, 2, 1024, 16, 12, 70
+    N, front = K + 1, -(-prefix // page)
+    pages = B * per + front
+    cos, sin = lfm.rope_tables(prefix + per * page)
+    weights = dev(r.standard_normal((V, 2048), dtype=np.float32) / 8)
+    qw, kw, dc, ds = dev(np.ones(64, np.float32)), dev(np.ones(64, np.float32)), dev(cos), dev(sin)
+    order = r.permutation(pages).astype(np.int32)
+    table, shared = dev(order[:B * per].reshape(B, per)), dev(order[B * per:])
+    start = r.standard_normal((2, pages, 8, page, 64)).astype(np.float16)
+    own = np.array([K + 1, 30, 100], np.int32)
+
+    class Side:
+        def __init__(self):
+            self.k, self.v = (dev(np.clip(a * 40, -127, 127).astype(np.int8)) for a in start)
+            self.ks, self.vs = (dev(np.full((pages, 8, page), 0.02, np.float32)) for _ in range(2))
+            self.c = lfm.KVCache(lfm.KV_INT8, pages, page, self.k, self.v, self.ks, self.vs)
+            self.len = dev(own)
+            self.b = lfm.KVBatch(B, self.len, table, per, max_new=N, max_len=128, prefix_pages=shared, prefix_len=prefix)
+            self.x, self.o = hip.DeviceArray((B * N, lfm.QKV_COLS)), hip.DeviceArray((B * N, 2048))
+            self.p, self.d = hip.DeviceArray((B * N, V)), hip.DeviceArray((B * K, V))
+            self.ids, self.acc, self.tok = (hip.DeviceArray(n, np.int32) for n in ((B, K), (B,), (B, N)))
+            self.ua, self.us = hip.DeviceArray((B, K)), hip.DeviceArray((B,))
+            self.need = [lfm.kv_attention_workspace(self.c, self.b), lfm.softmax_workspace(B * N, V),
+                         lfm.verify_draft_workspace(B, V)]
+            self.ws = hip.DeviceArray((max(self.need),), np.uint8)  # the calls follow one another
+
+        def step(self, st):
+            lfm.kv_write(self.c, self.b, self.x, lfm.QKV_COLS, q_weight=qw, k_weight=kw, cos=dc, sin=ds, max_pos=len(cos),
+                         stream=st)
+            lfm.kv_attention(self.c, self.b, self.x, lfm.QKV_COLS, self.o, workspace=self.ws,
+                             workspace_bytes=self.need[0], stream=st)
+            lfm.gemm_nt(self.o, weights, self.p, B * N, V, 2048, stream=st)
+            lfm.softmax(self.p, self.p, B * N, V, temperature=0.9, workspace=self.ws, workspace_bytes=self.need[1],
+                        stream=st)
+            lfm.verify_draft(self.p, self.d, self.ids, self.ua, self.us, self.acc, self.tok, B, K, V, workspace=self.ws,
+                             workspace_bytes=self.need[2], stream=st)
+
+    H, vp = hip.rt(), ctypes.c_void_p
+    graphed, eager, st = Side(), Side(), hip.Stream()
+    H.hipStreamBeginCapture.argtypes = [vp, ctypes.c_int]
+    H.hipStreamEndCapture.argtypes = [vp, ctypes.POINTER(vp)]
+    H.hipGraphInstantiate.argtypes = [ctypes.POINTER(vp), vp, vp, vp, ctypes.c_size_t]
+    H.hipGraphLaunch.argtypes = [vp, vp]
+    graph, ex = vp(), vp()
+    assert H.hipStreamBeginCapture(st.handle, 2) == 0
+    graphed.step(st)
+    assert H.hipStreamEndCapture(st.handle, ctypes.byref(graph)) == 0
+    assert H.hipGraphInstantiate(ctypes.byref(ex), graph, None, None, 0) == 0
+    for t in range(6):
+        x = r.standard_normal((B * N, lfm.QKV_COLS), dtype=np.float32)
+        ids, d = r.integers(0, V, (B, K)).astype(np.int32), np.full((B * K, V), 1.0 / V, np.float32)
+        ua, us = r.random((B, K), dtype=np.float32), r.random(B, dtype=np.float32)
+        for side in (graphed, eager):
+            for a, b in ((side.x, x), (side.d, d), (side.ids, ids), (side.ua, ua), (side.us, us), (side.len, own)):
+                a.upload(b)
+        assert H.hipGraphLaunch(ex, st.handle) == 0
+        st.synchronize()
+        eager.step(None)
+        hip.synchronize()
+        for a, b in ((graphed.o, eager.o), (graphed.p, eager.p), (graphed.acc, eager.acc), (graphed.tok, eager.tok),
+                     (graphed.k, eager.k), (graphed.vs, eager.vs)):
+            a, b = a.download(), b.download()
+            assert np.array_equal(a.view(np.uint8), b.view(np.uint8)), t
+        p = eager.p.download().reshape(B, N, V)
+        want = R.verify(p, d.reshape(B, K, V), ids, ua, us, np.full(B, K))
+        same((graphed.acc.download(), graphed.tok.download()), want)
+        own += want[0].astype(np.int32) + 1
+    H.hipGraphExecDestroy(ex)
+    H.hipGraphDestroy(graph)
