@@ -334,6 +334,21 @@ def test_attention_of_many_tiles_a_wave(fmt, heads, kv, page, new, own, prefix, 
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("fmt", FMTS)
+def test_pages_listed_more_than_once(fmt):
+    """Sequences that share pages with each other, with the prefix and with themselves."""
+    r = np.random.default_rng(fmt)
+    pool = Pool(fmt, 8, 16, 40)
+    q = Seqs(r, pool, [2, 1, 1], [90, 70, 33], prefix=40)
+    q.table[1, :4] = q.table[0, :4]  # positions 0 .. 63 alike
+    q.table[2, :2] = q.front[0]      # the prefix's first page, twice
+    q.d[1].upload(q.table)
+    fill(r, pool, q)
+    x = draws(r, (q.tokens, 2048), sizes=False)
+    check(pool, q, x, 32, attend(pool, q, x, 32))
+
+
+@pytest.mark.gpu
 def test_output_rows_of_their_own_length():
     from final_amd import hip, lfm
     r = np.random.default_rng(4)
