@@ -14,15 +14,14 @@ using moe::f32x4;
 // ---------------------------------------------------------------------------
 //
 // A row's maximum and its sum of exponentials under that maximum, in fp32, then
-// the quotients.  A thread keeps the values it loaded, so a row is read once
-// where a block takes a whole one; where that leaves CUs idle a row is split
-// over blocks that leave their maximum and sum in the workspace to a second
-// kernel, which reads the row again (from L2).  An exponential is 2 to the power of
-// the rounded difference times c = log2(e) / temperature: v_exp_f32 does it in one
-// instruction, where expf's 15 made a row's 65536 values 9 us of arithmetic.
-// Memory bounds many rows (320 of 65536, 168 MB: 45 us, 3.7 TB/s; the first 256, one
-// to a CU, read and then write all at once, 34 us, the other 64 split, 11), and the
-// chain load, maximum, sum, store a few (1 row: 7.8 us).
+// the quotients.  A block's threads keep the values they loaded, so a row of up to
+// 65536 is read once; longer rows are split over blocks that leave their maximum and
+// sum in the workspace to a second kernel, which reads the row again (from L2).  An
+// exponential is 2 to the power of the rounded difference times c = log2(e) /
+// temperature: v_exp_f32 does it in one instruction, where expf's 15 made a row's
+// 65536 values 9 us of arithmetic.  Memory bounds many rows (320 of 65536, 168 MB: 42
+// us, 4.0 TB/s; a CU holds one row, so the first 256 all read and then all write), and
+// the chain load, maximum, sum, store few (1 row: 6.9 us).
 
 constexpr int kSoftThreads = 1024;
 constexpr int kSoftRegs = 64;        // values a thread keeps
@@ -41,15 +40,18 @@ __device__ __forceinline__ float rescale(float m, float mx, float c) {
   return m == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f((m - mx) * c);
 }
 
-__device__ __forceinline__ float wave_max(float v) {
+// Over groups of N lanes.
+template <int N = 64>
+__device__ __forceinline__ float lanes_max(float v) {
 #pragma unroll
-  for (int d = 32; d > 0; d >>= 1) v = fmaxf(v, __shfl_xor(v, d));
+  for (int d = N / 2; d > 0; d >>= 1) v = fmaxf(v, __shfl_xor(v, d));
   return v;
 }
 
-__device__ __forceinline__ float wave_sum(float v) {
+template <int N = 64>
+__device__ __forceinline__ float lanes_sum(float v) {
 #pragma unroll
-  for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d);
+  for (int d = N / 2; d > 0; d >>= 1) v += __shfl_xor(v, d);
   return v;
 }
 
@@ -77,17 +79,15 @@ __device__ __forceinline__ void load_values(const float *x, int n, RowValues<NR>
   r.tail = tid < (n & 3) ? x[4 * groups + tid] : -__builtin_inff();
 }
 
-// Groups [j0, j1) of a thread's values times `scale`, and the tail where asked for.
 template <int NW, int NR>
-__device__ __forceinline__ void store_values(float *y, int n, const RowValues<NR> &r, float scale, int j0 = 0,
-                                             int j1 = NR / 4, bool tail = true) {
+__device__ __forceinline__ void store_values(float *y, int n, const RowValues<NR> &r, float scale) {
   const int groups = n >> 2, tid = threadIdx.x;
 #pragma unroll
   for (int j = 0; j < NR / 4; ++j) {
     const int i = j * NW * 64 + tid;
-    if (i < groups && j >= j0 && j < j1) *reinterpret_cast<f32x4_any *>(y + 4 * i) = r.v[j] * scale;
+    if (i < groups) *reinterpret_cast<f32x4_any *>(y + 4 * i) = r.v[j] * scale;
   }
-  if (tail && tid < (n & 3)) y[4 * groups + tid] = r.tail * scale;
+  if (tid < (n & 3)) y[4 * groups + tid] = r.tail * scale;
 }
 
 // The values become exp((v - ref) / t); their sum.  -infinity gives 0 whatever ref is.
@@ -105,57 +105,56 @@ __device__ __forceinline__ float exp_values(RowValues<NR> &r, float ref, float c
   return l;
 }
 
-// Maximum over a block of NW waves, then the sum of exponentials under it.
+// A block's maximum and its sum of exponentials under it.  The values become
+// exponentials under their thread's own maximum, with no barrier between loads and
+// exponentials, so that a wave's run while others still load; `mine` is what they
+// count under the block's.
 template <int NW, int NR>
-__device__ __forceinline__ MaxSum block_exp(RowValues<NR> &r, float c, float *s_part) {
-  const int wave = threadIdx.x >> 6;
+__device__ __forceinline__ MaxSum block_exp(RowValues<NR> &r, float c, float2 *s_part, float &mine) {
   float m = r.tail;
 #pragma unroll
   for (int j = 0; j < NR / 4; ++j)
 #pragma unroll
     for (int e = 0; e < 4; ++e) m = fmaxf(m, r.v[j][e]);
-  m = wave_max(m);
-  if ((threadIdx.x & 63) == 0) s_part[wave] = m;
+  float l = exp_values(r, m == -__builtin_inff() ? 0.0f : m, c);
+  float mx = lanes_max(m);
+  l = lanes_sum(l * rescale(m, mx, c));
+  if ((threadIdx.x & 63) == 0) s_part[threadIdx.x >> 6] = float2{mx, l};
   __syncthreads();
-  m = s_part[0];
-#pragma unroll
-  for (int w = 1; w < NW; ++w) m = fmaxf(m, s_part[w]);
-  float l = wave_sum(exp_values(r, m == -__builtin_inff() ? 0.0f : m, c));
-  if ((threadIdx.x & 63) == 0) s_part[NW + wave] = l;
-  __syncthreads();
-  l = s_part[NW];
-#pragma unroll
-  for (int w = 1; w < NW; ++w) l += s_part[NW + w];
-  return {m, l};
+  const float2 p = s_part[threadIdx.x & (NW - 1)];  // a wave's in each of NW lanes
+  mx = lanes_max<NW>(p.x);
+  l = lanes_sum<NW>(p.y * rescale(p.x, mx, c));
+  mine = rescale(m, mx, c);
+  return {mx, l};
 }
 
 __device__ __forceinline__ float inverse_sum(float l) { return l == 0.0f ? 0.0f : 1.0f / l; }
 
-// A row, NR values a thread; gridDim.y blocks each read all of it and write their
-// share.
+// A row a block, NR values a thread.
 template <int NR>
 __global__ __launch_bounds__(kSoftThreads) __attribute__((amdgpu_waves_per_eu(NR <= 32 ? 8 : 4)))
 void softmax_row_kernel(const float *x, long long xs, float *y, long long ys, int dim, float c) {
   constexpr int NW = kSoftThreads / 64;
-  __shared__ float s_part[2 * NW];
+  __shared__ float2 s_part[NW];
   x += blockIdx.x * xs;
   y += blockIdx.x * ys;
   RowValues<NR> v;
   load_values<NW, NR>(x, dim, v);
-  const MaxSum r = block_exp<NW, NR>(v, c, s_part);
-  const int share = NR / 4 / gridDim.y;
-  store_values<NW, NR>(y, dim, v, inverse_sum(r.l), blockIdx.y * share, (blockIdx.y + 1) * share, blockIdx.y == 0);
+  float mine;
+  const MaxSum r = block_exp<NW, NR>(v, c, s_part, mine);
+  store_values<NW, NR>(y, dim, v, mine * inverse_sum(r.l));
 }
 
 // A slice of a row a block: its maximum and sum.
 __global__ __launch_bounds__(kSliceThreads) void softmax_part_kernel(const float *x, long long xs, float2 *part, int dim,
                                                                      float c) {
   constexpr int NW = kSliceThreads / 64;
-  __shared__ float s_part[2 * NW];
+  __shared__ float2 s_part[NW];
   const int first = blockIdx.x * kSlice, n = min(dim - first, kSlice);
   RowValues<kSliceRegs> v;
   load_values<NW, kSliceRegs>(x + blockIdx.y * xs + first, n, v);
-  const MaxSum r = block_exp<NW, kSliceRegs>(v, c, s_part);
+  float mine;
+  const MaxSum r = block_exp<NW, kSliceRegs>(v, c, s_part, mine);
   if (threadIdx.x == 0) part[(size_t)blockIdx.y * gridDim.x + blockIdx.x] = float2{r.m, r.l};
 }
 
@@ -170,46 +169,28 @@ __global__ __launch_bounds__(kSliceThreads) void softmax_finish_kernel(const flo
   const float2 *p = part + (size_t)blockIdx.y * gridDim.x;
   float m = -__builtin_inff();
   for (int i = lane; i < (int)gridDim.x; i += 64) m = fmaxf(m, p[i].x);
-  m = wave_max(m);
+  m = lanes_max(m);
   const float ref = m == -__builtin_inff() ? 0.0f : m;
   float l = 0.0f;
   for (int i = lane; i < (int)gridDim.x; i += 64) l += p[i].y * rescale(p[i].x, ref, c);
-  const float inv = inverse_sum(wave_sum(l));
+  const float inv = inverse_sum(lanes_sum(l));
   exp_values(v, ref, c);
   store_values<NW, kSliceRegs>(y + blockIdx.y * ys + first, n, v, inv);
 }
 
-// How many of the first rows take a block each.  Those of up to 8192 values all do;
-// of 32768, of which a CU holds two, from 128 rows; of 65536, of which it holds one,
-// full rounds of the CUs and a last one from 144 rows (65536 values, a block a row /
-// split: 128 rows 16.3 / 16.8 us, 160 rows 17.7 / 23.2, 256 rows 25.6 / 36).
-constexpr int kShortRow = 8 * kSoftThreads, kMidRow = 32 * kSoftThreads, kSoftCUs = 256;
-
-static int whole_rows(int rows, int dim) {
-  if (dim <= kShortRow) return rows;
-  if (dim > kSoftRow) return 0;
-  if (dim <= kMidRow) return rows >= 128 ? rows : 0;
-  const int left = rows % kSoftCUs;
-  return left >= 144 ? rows : rows - left;
-}
-
-// Whether the others share the CUs' blocks out between them, each block reading a
-// whole row, where nobody overwrites what another has to read (y is not x): one
-// launch instead of two (1 row of 65536: 8.0 us, split 6.5 and a launch; 64 rows of
-// 32000: 7.8 / 8.2; 64 rows of 65536 from HBM 18 / 12).
-constexpr int kShareRows = 32;
-
-static bool share_rows(int left, int whole, int dim) {
-  return dim <= kMidRow || (dim <= kSoftRow && whole == 0 && left <= kShareRows);
-}
+// A row of up to kSoftRow values is one block's, however few the rows: split over
+// blocks that leave their sums to a second launch, 1 row of 65536 takes 6.5 us and 8
+// blocks that read it all and write an eighth each 7.1, one block 6.9; 64 rows 12.0 /
+// 12.1 / 11.3, 320 rows 46 split, 42 in blocks, 43 with the last 64 split.
+constexpr int kShortRow = 8 * kSoftThreads, kMidRow = 32 * kSoftThreads;
 
 size_t softmax_ws(int rows, int dim) {
-  return (size_t)(rows - whole_rows(rows, dim)) * ((dim + kSlice - 1) / kSlice) * sizeof(float2);
+  return dim <= kSoftRow ? 0 : (size_t)rows * ((dim + kSlice - 1) / kSlice) * sizeof(float2);
 }
 
-static void softmax_rows_launch(const float *x, long long xs, float *y, long long ys, int rows, int share, int dim,
-                                float c, hipStream_t st) {
-  const dim3 grid(rows, share), block(kSoftThreads);
+static void softmax_rows_launch(const float *x, long long xs, float *y, long long ys, int rows, int dim, float c,
+                                hipStream_t st) {
+  const dim3 grid(rows), block(kSoftThreads);
   if (dim <= kShortRow)
     hipLaunchKernelGGL(softmax_row_kernel<8>, grid, block, 0, st, x, xs, y, ys, dim, c);
   else if (dim <= kMidRow)
@@ -221,22 +202,16 @@ static void softmax_rows_launch(const float *x, long long xs, float *y, long lon
 hipError_t launch_softmax(const float *x, long long xs, float *y, long long ys, int rows, int dim,
                           float temperature, void *ws, hipStream_t st) {
   const float c = (float)(1.4426950408889634 / (double)temperature);
-  const int whole = whole_rows(rows, dim), left = rows - whole;
-  constexpr int kMostRows = 1 << 21;  // of a launch: its threads are counted in 32 bits
-  for (long long r0 = 0; r0 < whole; r0 += kMostRows)
-    softmax_rows_launch(x + r0 * xs, xs, y + r0 * ys, ys, (int)std::min<long long>(whole - r0, kMostRows), 1, dim, c, st);
-  x += whole * xs;
-  y += whole * ys;
-  if (left > 0 && x != y && share_rows(left, whole, dim)) {
-    int share = 1;
-    while (share < 8 && 2 * share * left <= kSoftCUs) share *= 2;
-    softmax_rows_launch(x, xs, y, ys, left, share, dim, c, st);
+  if (dim <= kSoftRow) {
+    constexpr int kMostRows = 1 << 21;  // of a launch: its threads are counted in 32 bits
+    for (long long r0 = 0; r0 < rows; r0 += kMostRows)
+      softmax_rows_launch(x + r0 * xs, xs, y + r0 * ys, ys, (int)std::min<long long>(rows - r0, kMostRows), dim, c, st);
     return hipGetLastError();
   }
   const int slices = (dim + kSlice - 1) / kSlice;
   float2 *part = static_cast<float2 *>(ws);
-  for (int r0 = 0; r0 < left; r0 += 65535) {  // rows a launch may have
-    const dim3 grid(slices, std::min(left - r0, 65535));
+  for (long long r0 = 0; r0 < rows; r0 += 65535) {  // rows a launch may have
+    const dim3 grid(slices, (unsigned)std::min<long long>(rows - r0, 65535));
     float2 *p = part + (size_t)r0 * slices;
     hipLaunchKernelGGL(softmax_part_kernel, grid, dim3(kSliceThreads), 0, st, x + r0 * xs, xs, p, dim, c);
     hipLaunchKernelGGL(softmax_finish_kernel, grid, dim3(kSliceThreads), 0, st, x + r0 * xs, xs, y + r0 * ys, ys, p, dim,

@@ -195,8 +195,7 @@ int lfm_kv_attention_workspace(const lfm_kv_cache *cache, const lfm_kv_batch *ba
  * logits of `rows` rows of `dim`, row r at x + r*x_stride and y + r*y_stride
  * (floats).  A logit of -infinity gives 0, a row of nothing else zeros; NaN or
  * +infinity makes its row NaN.  temperature from 2^-120 to 2^120.  y may be
- * x (with equal strides; the sums may then be taken in another order); otherwise
- * the two do not overlap.  workspace: lfm_softmax_workspace bytes, as for
+ * x (with equal strides); otherwise the two do not overlap.  workspace: lfm_softmax_workspace bytes, as for
  * lfm_kv_attention. */
 int lfm_softmax(const float *x, long long x_stride, float *y, long long y_stride, int rows, int dim,
                 float temperature, void *workspace, size_t workspace_bytes, moe_stream_t stream);
