@@ -19,8 +19,8 @@ using moe::f32x4;
 // sum in the workspace to a second kernel, which reads the row again (from L2).  An
 // exponential is 2 to the power of the rounded difference times c = log2(e) /
 // temperature: v_exp_f32 does it in one instruction, where expf's 15 made a row's
-// 65536 values 9 us of arithmetic.  Memory bounds many rows (320 of 65536, 168 MB: 42
-// us, 4.0 TB/s; a CU holds one row, so the first 256 all read and then all write), and
+// 65536 values 9 us of arithmetic.  Memory bounds many rows (320 of 65536, 168 MB: 33
+// us, 5.1 TB/s; a CU holds one row, so the first 256 all read and then all write), and
 // the chain load, maximum, sum, store few (1 row: 6.9 us).
 
 constexpr int kSoftThreads = 1024;
@@ -79,13 +79,18 @@ __device__ __forceinline__ void load_values(const float *x, int n, RowValues<NR>
   r.tail = tid < (n & 3) ? x[4 * groups + tid] : -__builtin_inff();
 }
 
+// Stores past the caches, so that the logits, which the head has just written, are not
+// driven out of the last one (256 MB) while they are read: 320 rows of 65536 take 33
+// us instead of 41 where they are there, 39 either way where they come from HBM.  A copy
+// of the logits, this and verification of 64 x 5 rows together 77 us instead of 84
+// (in place 76 either way).
 template <int NW, int NR>
 __device__ __forceinline__ void store_values(float *y, int n, const RowValues<NR> &r, float scale) {
   const int groups = n >> 2, tid = threadIdx.x;
 #pragma unroll
   for (int j = 0; j < NR / 4; ++j) {
     const int i = j * NW * 64 + tid;
-    if (i < groups) *reinterpret_cast<f32x4_any *>(y + 4 * i) = r.v[j] * scale;
+    if (i < groups) __builtin_nontemporal_store(f32x4_any(r.v[j] * scale), reinterpret_cast<f32x4_any *>(y + 4 * i));
   }
   if (tid < (n & 3)) y[4 * groups + tid] = r.tail * scale;
 }
@@ -181,7 +186,8 @@ __global__ __launch_bounds__(kSliceThreads) void softmax_finish_kernel(const flo
 // A row of up to kSoftRow values is one block's, however few the rows: split over
 // blocks that leave their sums to a second launch, 1 row of 65536 takes 6.5 us and 8
 // blocks that read it all and write an eighth each 7.1, one block 6.9; 64 rows 12.0 /
-// 12.1 / 11.3, 320 rows 46 split, 42 in blocks, 43 with the last 64 split.
+// 12.1 / 11.3, 320 rows 46 split, 42 in blocks, 43 with the last 64 split (all with
+// stores through the caches).
 constexpr int kShortRow = 8 * kSoftThreads, kMidRow = 32 * kSoftThreads;
 
 size_t softmax_ws(int rows, int dim) {
