@@ -911,6 +911,16 @@ static int widest(int format) { return format == LFM_KV_F32 ? 2 : 4; }
 // A tile's time, to that of one column tile.
 static float tile_cost(int ct) { return ct <= 1 ? 1.0f : ct == 2 ? 1.6f : 2.8f; }
 
+// Tiles below which own positions with no prefix beside them are not split: the parts'
+// join is a second launch, 4 to 5 us.  By the call's longest sequence, since it waits for
+// the slowest.  8 sequences, us unsplit / split: 1 token over int8 900 positions 9.8 / 14.0,
+// 2000 14.0 / 14.4, 3000 17.9 / 15; bf16 900 10.9 / 13.8, 2000 16.4 / 16.8; fp32 700 14.4 /
+// 16.4, 1500 21 / 17; 5 tokens over int8 550 10.9 / 15.3, 1500 18.4 / 16.2; 20 tokens 550
+// 16.2 / 17.2, 1500 27.8 / 17.8.
+static int whole_tiles(int format, int ct) {
+  return own_waves(ct) * (format == LFM_KV_F32 ? 4 : ct <= 2 ? 8 : 5);
+}
+
 static FlashPlan flash_plan(const KvArgs &a, int heads) {
   FlashPlan p{};
   const long long group = heads / a.kv_heads, cap = (long long)a.max_pages << a.pshift;
@@ -923,6 +933,7 @@ static FlashPlan flash_plan(const KvArgs &a, int heads) {
   const int most = active_parts(keys, kMostParts);
   const float own_time = (float)keys * tile_cost(p.own_ct);  // of a wave
   if (a.prefix_len == 0) {
+    if ((keys + kKeys - 1) / kKeys < whole_tiles(a.format, p.own_ct)) return p;
     const long long slots = kFlashCUs * flash_waves(a.format, p.own_ct) * 4 / own_waves(p.own_ct);
     p.own_parts = (int)std::min<long long>(most, std::max<long long>(1, slots / own_base));
     return p;

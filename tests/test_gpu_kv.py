@@ -334,6 +334,19 @@ def test_attention_of_many_tiles_a_wave(fmt, heads, kv, page, new, own, prefix, 
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("fmt,new,longest", [(R.F32, 1, 992), (R.INT8, 1, 2016), (R.BF16, 3, 992), (R.FP8, 9, 608)])
+def test_attention_around_the_length_that_is_split(fmt, new, longest):
+    r = np.random.default_rng(longest)
+    pool = Pool(fmt, 8, 32, 140)
+    for own in (longest, longest + 1):
+        say(f"[kv attention] fmt={fmt} new={new} own={own}")
+        q = Seqs(r, pool, [new, new], [own, longest // 2])
+        fill(r, pool, q)
+        x = draws(r, (q.tokens, 2048), sizes=False)
+        check(pool, q, x, 32, attend(pool, q, x, 32))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("fmt", FMTS)
 def test_pages_listed_more_than_once(fmt):
     """Sequences that share pages with each other, with the prefix and with themselves."""
