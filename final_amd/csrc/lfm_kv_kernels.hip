@@ -371,17 +371,21 @@ __device__ __forceinline__ void value_operands(const RawTile<FMT> &r, bf16x8 (&o
   }
 }
 
+// Which positions a block takes: a sequence's own, the shared prefix's for all
+// sequences, or a sequence's own with the prefix's tiles in front of them.
+enum FlashKeys { kOwnKeys, kPrefixKeys, kBothKeys };
+
 // One block's part of a product: columns col0 .. of kv head h, every `stride`-th
-// tile of the own positions of sequence b (or, PREFIX, of the shared ones).
-// Tiles are dealt to the parts' waves in turn, so that a wave knows its first
-// tile, and looks up its page, before it knows how long the sequence is.
-template <int FMT, int CT, bool PREFIX, int W>
+// tile of KEYS (of sequence b).  Tiles are dealt to the parts' waves in turn, so that
+// a wave knows its first tile, and looks up its page, before it knows how long the
+// sequence is.
+template <int FMT, int CT, FlashKeys KEYS, int W>
 __device__ __forceinline__ void flash_part(const KvArgs &a, const FlashArgs &f, int h, int part, int group, int b,
                                            float *s_lds) {
   using Raw = RawTile<FMT>;
   using SH = FlashShape<CT, W>;
   constexpr int NP = FMT == LFM_KV_F32 ? 3 : 1, NT = SH::NT, COLS = SH::COLS, QP = SH::QP;
-  constexpr bool FEW = SH::FEW;
+  constexpr bool FEW = SH::FEW, PREFIX = KEYS == kPrefixKeys, BOTH = KEYS == kBothKeys;
   // q's parts as operands [column tile][k-step][part][lane], then the waves' sums
   bf16x8 *const s_q = reinterpret_cast<bf16x8 *>(s_lds);
   float2 *const s_m = reinterpret_cast<float2 *>(s_lds + SH::kFloats);  // [W][COLS]
@@ -391,10 +395,16 @@ __device__ __forceinline__ void flash_part(const KvArgs &a, const FlashArgs &f, 
   const int col0 = group * COLS;
   const int t0 = part * W + wave;
 
-  const int *table = PREFIX ? a.prefix_pages : a.pages + (size_t)b * a.max_pages;
-  const int most_pages = PREFIX ? (a.prefix_len - 1) >> a.pshift : a.max_pages - 1;
+  // tiles of the prefix in front of the own ones; a tile's number among its own kind
+  const int front = BOTH ? (a.prefix_len + kKeys - 1) / kKeys : 0;
+  auto in_front = [&](int t) { return BOTH && t < front; };
+  auto number = [&](int t) { return in_front(t) ? t : t - front; };
+  const int *own_table = a.pages + (size_t)b * a.max_pages;
+  auto table_of = [&](int t) { return PREFIX || in_front(t) ? a.prefix_pages : own_table; };
+  const int most_pages = PREFIX || in_front(t0) ? (a.prefix_len - 1) >> a.pshift : a.max_pages - 1;
   int first_pages = 0;  // of the first tile's halves, in lanes 0 and 1
-  if (most_pages >= 0) first_pages = table[min((t0 * kKeys + 16 * (lane & 1)) >> a.pshift, most_pages)];
+  if (most_pages >= 0)
+    first_pages = table_of(t0)[min((number(t0) * kKeys + 16 * (lane & 1)) >> a.pshift, most_pages)];
   KvSeq s;
   int len, first_seen;  // keys; those below first_seen are seen by every column of the block
   if (PREFIX) {
@@ -411,7 +421,8 @@ __device__ __forceinline__ void flash_part(const KvArgs &a, const FlashArgs &f, 
   const bool direct = !PREFIX && f.prefix_parts == 0 && parts == 1;
   // the last position a column of the block sees
   const int seen = PREFIX ? len : min(len, len - s.n + (col0 + COLS - 1) / f.group + 1);
-  const int t_end = (seen + kKeys - 1) / kKeys;
+  const int t_end = front + (seen + kKeys - 1) / kKeys;
+  auto keys_of = [&](int t) { return in_front(t) ? a.prefix_len : len; };
 
   // q, for the column tiles' k-steps w, w + W, ... in wave w
   constexpr int QE = (2 * NT + W - 1) / W;
@@ -435,7 +446,7 @@ __device__ __forceinline__ void flash_part(const KvArgs &a, const FlashArgs &f, 
 #pragma unroll
     for (int hb = 0; hb < 2; ++hb) {
       // a half tile behind the last key repeats the one with that key
-      const int k0 = min(t * kKeys + 16 * hb, (len - 1) & ~15), page = hb ? page1 : page0;
+      const int k0 = min(number(t) * kKeys + 16 * hb, (keys_of(t) - 1) & ~15), page = hb ? page1 : page0;
       r.ok[hb] = page >= 0;
       const size_t row = kv_row(a, max(page, 0), h, k0 & ((1 << a.pshift) - 1));
       // the half tile's 16 rows as buffers: a scalar base, and offsets of the lane alone
@@ -470,7 +481,8 @@ __device__ __forceinline__ void flash_part(const KvArgs &a, const FlashArgs &f, 
   };
   // Pages of 32 of the wave's tiles, a half tile's in each lane (-1 outside the cache).
   auto page_of = [&](int t) {
-    return table[min((t + stride * (lane >> 1)) * kKeys + 16 * (lane & 1), (len - 1) & ~15) >> a.pshift];
+    t += stride * (lane >> 1);
+    return table_of(t)[min(number(t) * kKeys + 16 * (lane & 1), (keys_of(t) - 1) & ~15) >> a.pshift];
   };
 
   f32x4 o[NT][4];
@@ -487,10 +499,11 @@ __device__ __forceinline__ void flash_part(const KvArgs &a, const FlashArgs &f, 
   // Tile t from r, while `next` (on pages next0 and next1) is loaded to rn.  The
   // values become operands after the scores, for the registers.
   auto tile = [&](int t, Raw &r, Raw &rn, int next, int next0, int next1) {
-    const int k0 = t * kKeys;
+    const int k0 = number(t) * kKeys;
+    auto last_of = [&](int ct) { return in_front(t) ? a.prefix_len - 1 : last[ct]; };
     const bool ok[2] = {r.ok[0], r.ok[1]};
     // some keys are behind the end, behind a column's own position or on no page (wave-uniform)
-    const bool cut = k0 + kKeys > first_seen || !ok[0] || !ok[1];
+    const bool cut = k0 + kKeys > (in_front(t) ? a.prefix_len : first_seen) || !ok[0] || !ok[1];
     if constexpr (Raw::SCALED) {
       // or the compiler takes the bytes apart as they arrive, in three steps each
 #pragma unroll
@@ -527,7 +540,7 @@ __device__ __forceinline__ void flash_part(const KvArgs &a, const FlashArgs &f, 
       for (int ct = 0; ct < NT; ++ct)
 #pragma unroll
         for (int e = 0; e < 8; ++e)
-          p[ct][e] = !ok[e >> 2] || k0 + 16 * (e >> 2) + 4 * g + (e & 3) > last[ct] ? kNoScore : p[ct][e];
+          p[ct][e] = !ok[e >> 2] || k0 + 16 * (e >> 2) + 4 * g + (e & 3) > last_of(ct) ? kNoScore : p[ct][e];
     }
     bool raise = false;
 #pragma unroll
@@ -631,7 +644,7 @@ __device__ __forceinline__ void flash_part(const KvArgs &a, const FlashArgs &f, 
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int k = k0 + 16 * (j >> 1) + 4 * g + 2 * (j & 1);
-          see[j] = (k <= last[ct] ? 0x3F80u : 0u) | (k + 1 <= last[ct] ? 0x3F800000u : 0u);
+          see[j] = (k <= last_of(ct) ? 0x3F80u : 0u) | (k + 1 <= last_of(ct) ? 0x3F800000u : 0u);
           see[j] = ok[j >> 1] ? see[j] : 0u;
         }
 #pragma unroll
@@ -654,7 +667,7 @@ __device__ __forceinline__ void flash_part(const KvArgs &a, const FlashArgs &f, 
   if (t0 < t_end) {
     pages = kv_page(a, page_of(t0));
     const int half0 = __builtin_amdgcn_readlane(first_pages, 0);
-    const int half1 = t0 * kKeys + 16 < len ? __builtin_amdgcn_readlane(first_pages, 1) : half0;
+    const int half1 = number(t0) * kKeys + 16 < keys_of(t0) ? __builtin_amdgcn_readlane(first_pages, 1) : half0;
     load(t0, kv_page(a, half0), kv_page(a, half1), ra);
   }
   // q's parts, scaled so that a score is the log2 of its weight
@@ -755,13 +768,13 @@ __device__ __forceinline__ void flash_part(const KvArgs &a, const FlashArgs &f, 
 // Waves a SIMD holds, by the registers a tile's columns take.
 constexpr int flash_waves(int fmt, int ct) { return fmt == LFM_KV_F32 ? 2 : ct == 0 ? 4 : ct == 1 ? 3 : 2; }
 
-// Own positions alone.  kv head fastest: with 8 of them a head's keys stay in one
-// XCD's L2.
-template <int FMT, int CT>
+// A sequence's positions alone.  kv head fastest: with 8 of them a head's keys stay in
+// one XCD's L2.
+template <int FMT, int CT, FlashKeys KEYS>
 __global__ __launch_bounds__(64 * own_waves(CT)) __attribute__((amdgpu_waves_per_eu(flash_waves(FMT, CT))))
 void kv_flash_kernel(KvArgs a, FlashArgs f) {
   __shared__ float s_lds[FlashShape<CT, own_waves(CT)>::kBytes / 4];
-  flash_part<FMT, CT, false, own_waves(CT)>(a, f, blockIdx.x % a.kv_heads, blockIdx.x / a.kv_heads, blockIdx.y,
+  flash_part<FMT, CT, KEYS, own_waves(CT)>(a, f, blockIdx.x % a.kv_heads, blockIdx.x / a.kv_heads, blockIdx.y,
                                             blockIdx.z, s_lds);
 }
 
@@ -777,14 +790,14 @@ void kv_prefix_flash_kernel(KvArgs a, FlashArgs f, int prefix_blocks, int own_gr
   if (at < prefix_blocks) {
     const int h = at % a.kv_heads;
     at /= a.kv_heads;
-    flash_part<FMT, PCT, true, W>(a, f, h, at % f.prefix_parts, at / f.prefix_parts, 0, s_lds);
+    flash_part<FMT, PCT, kPrefixKeys, W>(a, f, h, at % f.prefix_parts, at / f.prefix_parts, 0, s_lds);
   } else {
     at -= prefix_blocks;
     const int h = at % a.kv_heads;
     at /= a.kv_heads;
     const int part = at % f.own_parts;
     at /= f.own_parts;
-    flash_part<FMT, CT, false, W>(a, f, h, part, at % own_groups, at / own_groups, s_lds);
+    flash_part<FMT, CT, kOwnKeys, W>(a, f, h, part, at % own_groups, at / own_groups, s_lds);
   }
 }
 
@@ -911,12 +924,16 @@ static int widest(int format) { return format == LFM_KV_F32 ? 2 : 4; }
 // A tile's time, to that of one column tile.
 static float tile_cost(int ct) { return ct <= 1 ? 1.0f : ct == 2 ? 1.6f : 2.8f; }
 
-// Tiles below which own positions with no prefix beside them are not split: the parts'
-// join is a second launch, 4 to 5 us.  By the call's longest sequence, since it waits for
-// the slowest.  8 sequences, us unsplit / split: 1 token over int8 900 positions 9.8 / 14.0,
-// 2000 14.0 / 14.4, 3000 17.9 / 15; bf16 900 10.9 / 13.8, 2000 16.4 / 16.8; fp32 700 14.4 /
-// 16.4, 1500 21 / 17; 5 tokens over int8 550 10.9 / 15.3, 1500 18.4 / 16.2; 20 tokens 550
-// 16.2 / 17.2, 1500 27.8 / 17.8.
+// Tiles of a block below which a sequence's positions are not split, nor the prefix
+// shared (each sequence then reads it for itself): the parts' join is a second launch, 4
+// to 5 us and what the host takes.  By the call's longest sequence, since it waits for the
+// slowest; for blocks that have a CU to themselves, half of it where two share one.  8
+// sequences, us in one launch / two: 1 token over int8 900 positions 9.8 / 14.0, 2000 14.0
+// / 14.4, 3000 17.9 / 15; bf16 900 10.9 / 13.8, 2000 16.4 / 16.8; fp32 700 14.4 / 16.4,
+// 1500 21 / 17; 5 tokens over int8 550 10.9 / 15.3, 1500 18.4 / 16.2; 20 tokens 550 16.2 /
+// 17.2, 1500 27.8 / 17.8.  1 token over 300 int8 positions behind 700 shared 10.4 / 16.8,
+// 700 behind 1700 15.6 / 16.3, 100 behind 3000 18.5 / 16.6; 64 sequences of 300 bf16
+// behind 1200 23.1 / 18.7, 100 behind 300 12.7 / 17.2.
 static int whole_tiles(int format, int ct) {
   return own_waves(ct) * (format == LFM_KV_F32 ? 4 : ct <= 2 ? 8 : 5);
 }
@@ -932,10 +949,12 @@ static FlashPlan flash_plan(const KvArgs &a, int heads) {
   const long long own_base = (long long)p.own_groups * a.kv_heads * std::max(a.batch, 1);
   const int most = active_parts(keys, kMostParts);
   const float own_time = (float)keys * tile_cost(p.own_ct);  // of a wave
+  const long long own_slots = kFlashCUs * flash_waves(a.format, p.own_ct) * 4 / own_waves(p.own_ct);
+  const int tiles = (keys + kKeys - 1) / kKeys + (a.prefix_len + kKeys - 1) / kKeys;
+  if (own_base <= own_slots && tiles * ((own_base + kFlashCUs - 1) / kFlashCUs) < whole_tiles(a.format, p.own_ct))
+    return p;
   if (a.prefix_len == 0) {
-    if ((keys + kKeys - 1) / kKeys < whole_tiles(a.format, p.own_ct)) return p;
-    const long long slots = kFlashCUs * flash_waves(a.format, p.own_ct) * 4 / own_waves(p.own_ct);
-    p.own_parts = (int)std::min<long long>(most, std::max<long long>(1, slots / own_base));
+    p.own_parts = (int)std::min<long long>(most, std::max<long long>(1, own_slots / own_base));
     return p;
   }
   p.prefix_ct = all <= 16 && p.own_ct <= 1 ? 1 : widest(a.format);
@@ -991,9 +1010,11 @@ hipError_t launch_kv_attention(const KvArgs &a, const float *q, int ld, float *o
     constexpr int FMT = fmt(), MOST = FMT == LFM_KV_F32 ? 2 : 4;
     hipError_t e = by_columns<MOST>(p.own_ct, [&](auto own) -> hipError_t {
       constexpr int CT = own();
-      if (!p.prefix_parts)
-        hipLaunchKernelGGL((kv_flash_kernel<FMT, CT>), dim3(a.kv_heads * p.own_parts, p.own_groups, a.batch),
-                           dim3(64 * own_waves(CT)), 0, st, a, f);
+      const dim3 grid(a.kv_heads * p.own_parts, p.own_groups, a.batch), block(64 * own_waves(CT));
+      if (a.prefix_len == 0)
+        hipLaunchKernelGGL((kv_flash_kernel<FMT, CT, kOwnKeys>), grid, block, 0, st, a, f);
+      else if (p.prefix_parts == 0)
+        hipLaunchKernelGGL((kv_flash_kernel<FMT, CT, kBothKeys>), grid, block, 0, st, a, f);
       else if (p.prefix_ct == 1)
         hipLaunchKernelGGL((kv_prefix_flash_kernel<FMT, 1, CT < 1 ? CT : 1>), dim3((unsigned)(prefix_blocks + own_blocks)),
                            dim3(256), 0, st, a, f, (int)prefix_blocks, p.own_groups);

@@ -177,8 +177,8 @@ int lfm_kv_read(const lfm_kv_cache *cache, const lfm_kv_batch *batch, float *k_o
  * [tokens][ld], out has rows of ld_out.  heads a multiple of kv_heads, at most
  * 64 of them for each.  out does not overlap the columns that q is read from.  A
  * token that sees no position (its pages are outside the cache) gets zeros.  The
- * prefix's keys and values are read once for all sequences.  Sums, maxima and weights
- * are fp32.  A key that is not finite makes the outputs of the tokens that see
+ * keys and values of a prefix that is long enough are read once for all sequences.
+ * Sums, maxima and weights are fp32.  A key that is not finite makes the outputs of the tokens that see
  * it, for its heads, NaN, and a value that is not finite those of its column
  * not finite; what a token does not see does not reach it.
  * workspace: lfm_kv_attention_workspace bytes, 16-byte aligned (NULL where that

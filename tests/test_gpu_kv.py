@@ -296,7 +296,11 @@ CASES = [  # heads, kv, page, new, own, prefix
     (32, 8, 16, [1] * 70, list(range(1, 71)), 40), (12, 1, 16, [1], [4000], 0),
     # one to four column tiles of own positions, alone, beside a prefix of one column tile and of several
     (32, 8, 16, [3], [100], 70), (32, 8, 32, [3, 2], [100, 600], 300), (32, 8, 16, [6, 2], [9, 700], 0),
-    (32, 8, 16, [4], [600], 0), (16, 8, 64, [1, 2, 1], [600, 2, 31], 1500), (64, 8, 16, [2], [40], 2100)]
+    (32, 8, 16, [4], [600], 0), (16, 8, 64, [1, 2, 1], [600, 2, 31], 1500), (64, 8, 16, [2], [40], 2100),
+    # prefixes long enough to be shared, where those above are read by each sequence
+    (32, 8, 16, [1, 1, 1], [7, 150, 16], 2129), (32, 8, 64, [5, 3, 0, 8], [5, 200, 9, 64], 1033),
+    (5, 5, 16, [17, 16], [17, 90], 1115), (16, 2, 32, [4, 1], [100, 2], 2064), (64, 1, 16, [2], [77], 648),
+    (32, 8, 32, [1], [1], 2048), (32, 8, 16, [1] * 70, list(range(1, 71)), 1200)]
 
 
 @pytest.mark.gpu
@@ -415,12 +419,13 @@ def test_pages_beyond_4_gib(fmt):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("prefix", [100, 2100])  # read by each sequence, and shared
 @pytest.mark.parametrize("fmt", FMTS)
-def test_attention_of_large_scores(fmt):
+def test_attention_of_large_scores(fmt, prefix):
     """Scores of a few hundred, of either sign, values of magnitudes 2^-20 to 2^20."""
     r = np.random.default_rng(fmt)
-    pool = Pool(fmt, 8, 16, 60)
-    q = Seqs(r, pool, [3, 1], [90, 200], prefix=100)
+    pool = Pool(fmt, 8, 16, 190)
+    q = Seqs(r, pool, [3, 1], [90, 200], prefix=prefix)
     fill(r, pool, q, sizes=True)
     x = np.ldexp(draws(r, (q.tokens, 2048), sizes=False), -14).astype(np.float32)
     check(pool, q, x, 32, attend(pool, q, x, 32))
@@ -431,12 +436,13 @@ def test_attention_of_large_scores(fmt):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("prefix", [40, 2090])
 @pytest.mark.parametrize("fmt", FMTS)
-def test_attention_does_not_see_the_future(fmt):
+def test_attention_does_not_see_the_future(fmt, prefix):
     """What stands behind a token's own position, not finite ones included, changes none of its bits."""
     r = np.random.default_rng(fmt)
-    pool = Pool(fmt, 8, 16, 40)
-    q = Seqs(r, pool, [4, 3], [50, 35], prefix=40)
+    pool = Pool(fmt, 8, 16, 170)
+    q = Seqs(r, pool, [4, 3], [50, 35], prefix=prefix)
     fill(r, pool, q)
     x = draws(r, (q.tokens, 2048), sizes=False)
     clean = attend(pool, q, x, 32)
@@ -456,12 +462,12 @@ def test_attention_does_not_see_the_future(fmt):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("fmt", FMTS)
-@pytest.mark.parametrize("at", [3, 39])
-def test_not_finite_rows_reach_who_sees_them(fmt, at):
+@pytest.mark.parametrize("prefix,at", [(40, 3), (40, 39), (2090, 3), (2090, 2089)])
+def test_not_finite_rows_reach_who_sees_them(fmt, prefix, at):
     """A row of the prefix reaches every token; one of a kv head's keys or values only its heads."""
     r = np.random.default_rng(fmt)
-    pool = Pool(fmt, 8, 16, 40)
-    q = Seqs(r, pool, [4, 1], [50, 35], prefix=40)
+    pool = Pool(fmt, 8, 16, 170)
+    q = Seqs(r, pool, [4, 1], [50, 35], prefix=prefix)
     fill(r, pool, q)
     x = draws(r, (q.tokens, 2048), sizes=False)
     clean = attend(pool, q, x, 32)
@@ -487,10 +493,11 @@ def test_not_finite_rows_reach_who_sees_them(fmt, at):
 
 
 @pytest.mark.gpu
-def test_attention_of_not_finite_queries():
+@pytest.mark.parametrize("prefix", [40, 2090])
+def test_attention_of_not_finite_queries(prefix):
     r = np.random.default_rng(1)
-    pool = Pool(R.INT8, 8, 16, 40)
-    q = Seqs(r, pool, [2, 2], [50, 35], prefix=40)
+    pool = Pool(R.INT8, 8, 16, 170)
+    q = Seqs(r, pool, [2, 2], [50, 35], prefix=prefix)
     fill(r, pool, q)
     x = draws(r, (q.tokens, 2048), sizes=False)
     clean = attend(pool, q, x, 32)
@@ -502,30 +509,31 @@ def test_attention_of_not_finite_queries():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("prefix", [40, 2088])
 @pytest.mark.parametrize("fmt", FMTS)
-def test_pages_outside_the_cache(fmt):
+def test_pages_outside_the_cache(fmt, prefix):
     from final_amd import hip, lfm
     r = np.random.default_rng(fmt)
-    pool = Pool(fmt, 8, 16, 30)
-    q = Seqs(r, pool, [2, 1, 1], [70, 35, 16], prefix=40)
+    pool = Pool(fmt, 8, 16, 160)
+    q = Seqs(r, pool, [2, 1, 1], [70, 35, 16], prefix=prefix)
     fill(r, pool, q)
     x = draws(r, (q.tokens, lfm.QKV_COLS), sizes=False)
     table, front = q.table.copy(), q.front.copy()
-    table[0, 1], table[1, 2], table[2, 0], front[1] = 30, -1, 1 << 30, -(1 << 31)
+    table[0, 1], table[1, 2], table[2, 0], front[1] = pool.pages, -1, 1 << 30, -(1 << 31)
     q.d[1].upload(table)
     q.d[2].upload(front)
 
     def hide(b, n):
         j = np.arange(n) // 16
-        own = (np.arange(n) - 40) // 16
-        return np.where(np.arange(n) < 40, j == 1, own == [1, 2, 0][b])
+        own = (np.arange(n) - prefix) // 16
+        return np.where(np.arange(n) < prefix, j == 1, own == [1, 2, 0][b])
 
     flag = dev(np.zeros(1, np.int32))
     got = attend(pool, q, x, 32, flag=flag)
     assert flag.download()[0] == 1
     check(pool, q, x, 32, got, hide=hide)
     # nothing to see at all
-    front[:] = 99
+    front[:] = pool.pages + 69
     q.d[2].upload(front)
     assert not attend(pool, q, x, 32, flag=flag)[3].any()
     # reading back: zeros; writing: nothing
@@ -637,15 +645,16 @@ def test_steps_give_what_whole_sequences_give(batch, seq):
 
 
 @pytest.mark.gpu
-def test_graph_replays_follow_the_lengths():
+@pytest.mark.parametrize("prefix", [100, 2100])
+def test_graph_replays_follow_the_lengths(prefix):
     """write + attention captured once, replayed as sequences grow, with eager work between."""
     import ctypes
 
     from final_amd import hip, lfm
     r = np.random.default_rng(9)
     H, vp = hip.rt(), ctypes.c_void_p
-    pool, other = (Pool(R.FP8, 8, 16, 40) for _ in range(2))
-    q = Seqs(r, pool, [1, 1, 1], [20, 3, 40], prefix=100, uniform=True, max_pages=8, max_len=64)
+    pool, other = (Pool(R.FP8, 8, 16, 160) for _ in range(2))
+    q = Seqs(r, pool, [1, 1, 1], [20, 3, 40], prefix=prefix, uniform=True, max_pages=8, max_len=64)
     fill(r, pool, q)
     for i in range(2):
         other.data[i][...], other.scale[i][...] = pool.data[i], pool.scale[i]
