@@ -273,6 +273,24 @@ __device__ __forceinline__ double weight(float p, float q) {
   return d > 0.0 ? d : 0.0;
 }
 
+// Four of a row's neighbouring values a thread and step; 0 behind the row.
+template <int NW, int NR>
+__device__ __forceinline__ void load_weights(const float *x, int n, RowValues<NR> &r) {
+#pragma unroll
+  for (int j = 0; j < NR / 4; ++j) {
+    const int i = 4 * (j * NW * 64 + (int)threadIdx.x);
+    f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (i + 4 <= n) {
+      v = *reinterpret_cast<const f32x4_any *>(x + i);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 3; ++e)
+        if (i + e < n) v[e] = x[i + e];
+    }
+    r.v[j] = v;
+  }
+}
+
 struct DrawRow {
   const float *p, *q;  // q null: the target alone
 };
@@ -447,11 +465,126 @@ __global__ __launch_bounds__(kTokenThreads) void draw_token_kernel(VerifyArgs a,
   if (tid == 0 && a.n_draft == kTokenThreads) out[a.n_draft] = acc == a.n_draft ? token : -1;
 }
 
+// The same in one launch where a block's threads hold the row (and the draft's): four
+// ids a thread, 4096 a step of the block, so that a wave's four of a step are a segment
+// of 256 neighbouring ids.  Every wave finds the segment from the segments' sums, and
+// the one that holds it the id.  Calls one after the other, 64 sequences of 16384 ids: 5.0
+// us, of which the launch on the host is most, two launches 7.8.  With 32 ids a thread
+// (24000 to 32768) the registers do not hold the 64-bit sums as well: 10.3 us, two
+// launches 8.6.
+template <int NR>
+__global__ __launch_bounds__(kTokenThreads) void draw_whole_kernel(VerifyArgs a) {
+  constexpr int NW = kTokenThreads / 64, G = NR / 4, SEGS = G * NW, EACH = (SEGS + 63) / 64;
+  __shared__ double s_seg[SEGS];
+  __shared__ int s_token;
+  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const float u = a.u_sample[b];
+  const int n = drafts_of(a, b);
+  const int id = tid < a.n_draft ? a.ids[b * a.ids_stride + tid] : -1;
+  const int acc = accepted_drafts(a, b, n);
+  const DrawRow r = row_after(a, b, acc, n);
+  RowValues<NR> p, q;
+  load_weights<NW, NR>(r.p, a.vocab, p);
+  load_weights<NW, NR>(r.q ? r.q : r.p, r.q ? a.vocab : 0, q);  // zeros without one
+  bool use_rest = r.q != nullptr;
+  auto four = [&](int j, double (&w)[4]) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[e] = weight(p.v[j][e], q.v[j][e]);
+  };
+  double mine[EACH], sum, incl, total;
+  for (;;) {
+#pragma unroll
+    for (int j = 0; j < G; ++j) {
+      double w[4];
+      four(j, w);
+      const double seg = scan((w[0] + w[1]) + (w[2] + w[3]));
+      if (lane == 63) s_seg[j * NW + wave] = seg;
+      __builtin_amdgcn_sched_barrier(0);  // or every step's 64-bit sums are held at once, and spill
+    }
+    __syncthreads();
+    sum = 0.0;
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+      const int at = lane * EACH + i;
+      mine[i] = at < SEGS ? s_seg[at] : 0.0;
+      sum += mine[i];
+    }
+    incl = scan(sum);
+    total = lane_value(incl, 63);
+    if (!use_rest || total > 0.0) break;
+    use_rest = false;
+#pragma unroll
+    for (int j = 0; j < G; ++j) q.v[j] = f32x4(0.0f);
+    __syncthreads();
+  }
+  const double bar = (double)u * total;
+  const unsigned long long hit = __ballot(incl > bar && sum > 0.0);
+  int token = -1;
+  if (hit) {  // the same in every wave
+    const int at = __builtin_ctzll(hit);
+    double run = lane_value(incl - sum, at);
+    int seg = at * EACH;
+#pragma unroll
+    for (int i = 0; i < EACH - 1; ++i) {
+      const double next = run + lane_value(mine[i], at);
+      if (seg == at * EACH + i && !(next > bar)) {
+        run = next;
+        ++seg;
+      }
+    }
+    if (seg % NW == wave) {
+      double w[4] = {0.0, 0.0, 0.0, 0.0};
+#pragma unroll
+      for (int j = 0; j < G; ++j) {
+        asm("" : "+v"(p.v[j]));  // or the weights, of 64 bits each, are kept from above
+        if (j == seg / NW) four(j, w);
+      }
+      const double own = (w[0] + w[1]) + (w[2] + w[3]);
+      double upto = run + (scan(own) - own);
+      const int first = seg / NW * (4 * kTokenThreads) + 4 * tid;
+      int past = -1, last = -1;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        upto += w[e];
+        if (w[e] > 0.0) {
+          last = first + e;
+          if (past < 0 && upto > bar) past = first + e;
+        }
+      }
+      // the segment's sum was taken in another order: where only that passes the
+      // bar, the segment's last id it is
+      const unsigned long long is_past = __ballot(past >= 0), is_last = __ballot(last >= 0);
+      if (is_past)
+        token = __builtin_amdgcn_readlane(past, __builtin_ctzll(is_past));
+      else if (is_last)
+        token = __builtin_amdgcn_readlane(last, 63 - __builtin_clzll(is_last));
+      if (lane == 0) s_token = token;
+    }
+    __syncthreads();
+    token = s_token;
+  }
+  if (tid == 0) a.accepted[b] = acc;
+  int *out = a.tokens + (size_t)b * (a.n_draft + 1);
+  if (tid <= a.n_draft) out[tid] = tid < acc ? id : tid == acc ? token : -1;
+  if (tid == 0 && a.n_draft == kTokenThreads) out[a.n_draft] = acc == a.n_draft ? token : -1;
+}
+
+constexpr int kWholeVocab = 16 * kTokenThreads;  // ids of a row that a block holds
+
 size_t verify_draft_ws(int batch, int vocab) {
+  if (vocab <= kWholeVocab) return 0;
   return (size_t)batch * (((size_t)vocab + kDrawSlice - 1) / kDrawSlice) * sizeof(double2);
 }
 
 hipError_t launch_verify_draft(const VerifyArgs &a, void *ws, hipStream_t st) {
+  if (a.vocab <= kWholeVocab) {
+    const dim3 grid(a.batch), block(kTokenThreads);
+    if (a.vocab <= 8 * kTokenThreads)
+      hipLaunchKernelGGL(draw_whole_kernel<8>, grid, block, 0, st, a);
+    else
+      hipLaunchKernelGGL(draw_whole_kernel<16>, grid, block, 0, st, a);
+    return hipGetLastError();
+  }
   const int slices = (int)(((size_t)a.vocab + kDrawSlice - 1) / kDrawSlice);
   double2 *sums = static_cast<double2 *>(ws);
   hipLaunchKernelGGL(draw_sums_kernel, dim3(slices, a.batch), dim3(kDrawThreads), 0, st, a, sums);

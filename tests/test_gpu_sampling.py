@@ -144,7 +144,8 @@ def same(got, want):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("B,K,V", [(1, 0, 1), (1, 4, 65536), (3, 1, 2), (7, 3, 1001), (64, 4, 4096), (2, 8, 65537),
-                                   (5, 0, 150001), (300, 2, 700), (33, 16, 999)])
+                                   (5, 0, 150001), (300, 2, 700), (33, 16, 999), (3, 2, 8191), (3, 2, 8193), (2, 3, 16383),
+                                   (2, 3, 16384), (2, 3, 16385), (4, 0, 16384), (2, 1024, 40), (1, 1024, 17000)])
 def test_verify(B, K, V):
     say(f"[verify] B={B} K={K} V={V}")
     r = np.random.default_rng(B + K + V)
@@ -163,7 +164,7 @@ def test_verify(B, K, V):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("V", [5, 1000, 65536, 70001])
+@pytest.mark.parametrize("V", [5, 1000, 10001, 16384, 65536, 70001])
 def test_verify_borders(V):
     """Equal distributions, one-hot ones, zeros, random numbers at both ends, ids outside, NaN and negative weights."""
     r = np.random.default_rng(V)

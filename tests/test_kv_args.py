@@ -104,7 +104,7 @@ def test_softmax_and_verify_refused(lib):
         assert soft(**kw) == inv, kw
     assert soft(rows=0, x=None, y=None) == 0
 
-    def ver(target=A, draft=A, ids=A, stride=3, ua=A, us=A, b=2, k=3, v=10, acc=A, tok=A, ws=A, n=1 << 40):
+    def ver(target=A, draft=A, ids=A, stride=3, ua=A, us=A, b=2, k=3, v=40000, acc=A, tok=A, ws=A, n=1 << 40):
         return L.lfm_verify_draft(target, draft, ids, stride, ua, us, None, b, k, v, acc, tok, ws, n, None)
 
     for kw in (dict(target=None), dict(draft=None), dict(ids=None), dict(ua=None), dict(us=None), dict(acc=None),
