@@ -21,8 +21,8 @@ namespace lfm {
 // What bounds them is memory: every load that hangs on nothing but the sequence
 // stands in front, without a branch, pages and then R rows, so that four rows a
 // lane are in flight.  64 ragged sequences of up to 512 tokens and 8 heads in fp8 (117
-// MB): written in 33 us (3.5 TB/s, three quarters of it reads), read back in 23 us
-// (5.1 TB/s); 20011 bf16 tokens (123 MB) are read in 26 us.  A single token takes 2.4
+// MB): written in 32 us (3.7 TB/s, three quarters of it reads), read back in 21 us
+// (5.6 TB/s); 20011 bf16 tokens (123 MB) are read in 26 us.  A single token takes 2.4
 // and 37 take 3.1 us: a launch, and the table, page and row one after the other.
 
 // The page, or -1 (and the flag) where it is outside the cache.
@@ -32,12 +32,20 @@ __device__ __forceinline__ int kv_page(const KvArgs &a, int page) {
   return -1;
 }
 
+// Which of a sequence's `blocks` this one is, or `blocks` and more: block x is on XCD x % 8
+// (gridDim.x is a multiple of 8), and an XCD takes neighbouring rows, whose scales share
+// lines of 32 tokens (64 ragged fp8 prompts in and out: 34.0 + 22.7 us in block order).
+__device__ __forceinline__ int neighbours(int blocks) {
+  const int per = (blocks + 7) / 8, at = blockIdx.x >> 3;
+  return at < per ? (blockIdx.x & 7) * per + at : blocks;
+}
+
 template <int FMT, bool ROPE, int R>
 __global__ __launch_bounds__(256) void kv_write_kernel(KvArgs a, KvWriteArgs w) {
   KvSeq s;
   if (!kv_seq<true>(a, blockIdx.y, s)) return;
   const int qrows = ROPE ? w.heads : 0, per_tok = qrows + 2 * a.kv_heads, total = s.n * per_tok;
-  const int first = blockIdx.x * 16 * R;
+  const int first = neighbours((total + 16 * R - 1) / (16 * R)) * 16 * R;
   if (first >= total) return;
   const int c = threadIdx.x & 15, g = threadIdx.x >> 4;
   f32x4 x[R], cs[R], sn[R];
@@ -91,7 +99,7 @@ __global__ __launch_bounds__(256) void kv_read_kernel(KvArgs a, float *k_out, fl
   KvSeq s;
   if (!kv_seq<false>(a, blockIdx.y, s)) return;
   const int kinds = (k_out != nullptr) + (v_out != nullptr), per_pos = kinds * a.kv_heads;
-  const int total = min(s.len, rows) * per_pos, first = blockIdx.x * 16 * R;
+  const int total = min(s.len, rows) * per_pos, first = neighbours((total + 16 * R - 1) / (16 * R)) * 16 * R;
   if (first >= total) return;
   const int c = threadIdx.x & 15, g = threadIdx.x >> 4;
   int pos[R], row[R], page[R];
@@ -872,13 +880,15 @@ __global__ __launch_bounds__(256) void kv_join_kernel(KvArgs a, FlashArgs f) {
 // Rows a group of 16 lanes takes: four where they fill the CUs, else one.
 constexpr long long kSplitRows = 32768;
 
+static unsigned blocks_of(int rows, int each) { return ((unsigned)(rows + each - 1) / each + 7) / 8 * 8; }
+
 template <int FMT, bool ROPE>
 static hipError_t kv_write_launch(const KvArgs &a, const KvWriteArgs &w, hipStream_t st) {
   const int rows = a.max_new * ((ROPE ? w.heads : 0) + 2 * a.kv_heads);
   if ((long long)rows * a.batch <= kSplitRows)
-    hipLaunchKernelGGL((kv_write_kernel<FMT, ROPE, 1>), dim3((rows + 15) / 16, a.batch), dim3(256), 0, st, a, w);
+    hipLaunchKernelGGL((kv_write_kernel<FMT, ROPE, 1>), dim3(blocks_of(rows, 16), a.batch), dim3(256), 0, st, a, w);
   else
-    hipLaunchKernelGGL((kv_write_kernel<FMT, ROPE, 4>), dim3((rows + 63) / 64, a.batch), dim3(256), 0, st, a, w);
+    hipLaunchKernelGGL((kv_write_kernel<FMT, ROPE, 4>), dim3(blocks_of(rows, 64), a.batch), dim3(256), 0, st, a, w);
   return hipGetLastError();
 }
 
@@ -888,9 +898,9 @@ static hipError_t kv_read_launch(const KvArgs &a, float *k_out, float *v_out, in
                 ((k_out != nullptr) + (v_out != nullptr)) * a.kv_heads;
   if (n == 0) return hipSuccess;
   if ((long long)n * a.batch <= kSplitRows)
-    hipLaunchKernelGGL((kv_read_kernel<FMT, 1>), dim3((n + 15) / 16, a.batch), dim3(256), 0, st, a, k_out, v_out, rows, ld);
+    hipLaunchKernelGGL((kv_read_kernel<FMT, 1>), dim3(blocks_of(n, 16), a.batch), dim3(256), 0, st, a, k_out, v_out, rows, ld);
   else
-    hipLaunchKernelGGL((kv_read_kernel<FMT, 4>), dim3((n + 63) / 64, a.batch), dim3(256), 0, st, a, k_out, v_out, rows, ld);
+    hipLaunchKernelGGL((kv_read_kernel<FMT, 4>), dim3(blocks_of(n, 64), a.batch), dim3(256), 0, st, a, k_out, v_out, rows, ld);
   return hipGetLastError();
 }
 
