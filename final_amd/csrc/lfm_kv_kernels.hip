@@ -778,11 +778,11 @@ constexpr int flash_waves(int fmt, int ct) { return fmt == LFM_KV_F32 ? 2 : ct =
 
 // A sequence's positions alone.  kv head fastest: with 8 of them a head's keys stay in
 // one XCD's L2.
-template <int FMT, int CT, FlashKeys KEYS>
-__global__ __launch_bounds__(64 * own_waves(CT)) __attribute__((amdgpu_waves_per_eu(flash_waves(FMT, CT))))
+template <int FMT, int CT, FlashKeys KEYS, int W>
+__global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(flash_waves(FMT, CT))))
 void kv_flash_kernel(KvArgs a, FlashArgs f) {
-  __shared__ float s_lds[FlashShape<CT, own_waves(CT)>::kBytes / 4];
-  flash_part<FMT, CT, KEYS, own_waves(CT)>(a, f, blockIdx.x % a.kv_heads, blockIdx.x / a.kv_heads, blockIdx.y,
+  __shared__ float s_lds[FlashShape<CT, W>::kBytes / 4];
+  flash_part<FMT, CT, KEYS, W>(a, f, blockIdx.x % a.kv_heads, blockIdx.x / a.kv_heads, blockIdx.y,
                                             blockIdx.z, s_lds);
 }
 
@@ -936,6 +936,7 @@ hipError_t launch_kv_read(const KvArgs &a, float *k_out, float *v_out, int rows,
 // in 128: 34.9).
 struct FlashPlan {
   int own_ct, prefix_ct, own_groups, prefix_groups, own_parts, prefix_parts;
+  bool wide;  // own positions by blocks of kWideWaves
 };
 
 constexpr int kFlashCUs = 256, kMostParts = 256, kLongPrefix = 20480;
@@ -947,18 +948,24 @@ static int widest(int format) { return format == LFM_KV_F32 ? 2 : 4; }
 // A tile's time, to that of one column tile.
 static float tile_cost(int ct) { return ct <= 1 ? 1.0f : ct == 2 ? 1.6f : 2.8f; }
 
+// Waves of a block of column tiles that has a CU to itself: 5 tokens over 1000 int8
+// positions 12.6 us, 4 waves in two launches 16.2 (twice the 8 of a single token's blocks
+// wait for the CU's loads: 900 positions 10.7 us, 9.7 with 8).
+constexpr int kWideWaves = 8;
+
 // Tiles of a block below which a sequence's positions are not split, nor the prefix
 // shared (each sequence then reads it for itself): the parts' join is a second launch, 4
 // to 5 us and what the host takes.  By the call's longest sequence, since it waits for the
 // slowest; for blocks that have a CU to themselves, half of it where two share one.  8
 // sequences, us in one launch / two: 1 token over int8 900 positions 9.8 / 14.0, 2000 14.0
 // / 14.4, 3000 17.9 / 15; bf16 900 10.9 / 13.8, 2000 16.4 / 16.8; fp32 700 14.4 / 16.4,
-// 1500 21 / 17; 5 tokens over int8 550 10.9 / 15.3, 1500 18.4 / 16.2; 20 tokens 550 16.2 /
-// 17.2, 1500 27.8 / 17.8.  1 token over 300 int8 positions behind 700 shared 10.4 / 16.8,
-// 700 behind 1700 15.6 / 16.3, 100 behind 3000 18.5 / 16.6; 64 sequences of 300 bf16
-// behind 1200 23.1 / 18.7, 100 behind 300 12.7 / 17.2.
-static int whole_tiles(int format, int ct) {
-  return own_waves(ct) * (format == LFM_KV_F32 ? 4 : ct <= 2 ? 8 : 5);
+// 1500 21 / 17; 3 tokens over int8 1000 9.9 / 15.3, 1800 13.6 / 15.6, 5 tokens 1000 12.6 /
+// 16.2, 1800 17.5 / 16.3, 20 tokens 500 13.1 / 17, 1000 18.9 / 17.8; 5 tokens over fp32
+// 500 14.1 / 18.7, 900 20.1 / 17.4.  1 token over 300 int8 positions behind 700 shared
+// 10.4 / 16.8, 700 behind 1700 15.6 / 16.3, 100 behind 3000 18.5 / 16.6; 64 sequences of
+// 300 bf16 behind 1200 23.1 / 18.7, 100 behind 300 12.7 / 17.2.
+static int whole_tiles(int format, int ct, int waves) {
+  return waves * (format == LFM_KV_F32 ? (ct <= 1 ? 4 : 3) : ct <= 1 ? 8 : ct == 2 ? 6 : 3);
 }
 
 static FlashPlan flash_plan(const KvArgs &a, int heads) {
@@ -974,8 +981,11 @@ static FlashPlan flash_plan(const KvArgs &a, int heads) {
   const float own_time = (float)keys * tile_cost(p.own_ct);  // of a wave
   const long long own_slots = kFlashCUs * flash_waves(a.format, p.own_ct) * 4 / own_waves(p.own_ct);
   const int tiles = (keys + kKeys - 1) / kKeys + (a.prefix_len + kKeys - 1) / kKeys;
-  if (own_base <= own_slots && tiles * ((own_base + kFlashCUs - 1) / kFlashCUs) < whole_tiles(a.format, p.own_ct))
+  p.wide = p.own_ct > 0 && own_base <= kFlashCUs;
+  if (own_base <= own_slots && tiles * ((own_base + kFlashCUs - 1) / kFlashCUs) <
+                                   whole_tiles(a.format, p.own_ct, p.wide ? kWideWaves : own_waves(p.own_ct)))
     return p;
+  p.wide = false;
   if (a.prefix_len == 0) {
     p.own_parts = (int)std::min<long long>(most, std::max<long long>(1, own_slots / own_base));
     return p;
@@ -1033,11 +1043,16 @@ hipError_t launch_kv_attention(const KvArgs &a, const float *q, int ld, float *o
     constexpr int FMT = fmt(), MOST = FMT == LFM_KV_F32 ? 2 : 4;
     hipError_t e = by_columns<MOST>(p.own_ct, [&](auto own) -> hipError_t {
       constexpr int CT = own();
-      const dim3 grid(a.kv_heads * p.own_parts, p.own_groups, a.batch), block(64 * own_waves(CT));
-      if (a.prefix_len == 0)
-        hipLaunchKernelGGL((kv_flash_kernel<FMT, CT, kOwnKeys>), grid, block, 0, st, a, f);
+      constexpr int W = own_waves(CT), WIDE = CT == 0 ? W : kWideWaves;
+      const dim3 grid(a.kv_heads * p.own_parts, p.own_groups, a.batch), block(64 * (p.wide ? WIDE : W));
+      if (a.prefix_len == 0 && p.wide)
+        hipLaunchKernelGGL((kv_flash_kernel<FMT, CT, kOwnKeys, WIDE>), grid, block, 0, st, a, f);
+      else if (a.prefix_len == 0)
+        hipLaunchKernelGGL((kv_flash_kernel<FMT, CT, kOwnKeys, W>), grid, block, 0, st, a, f);
+      else if (p.wide)
+        hipLaunchKernelGGL((kv_flash_kernel<FMT, CT, kBothKeys, WIDE>), grid, block, 0, st, a, f);
       else if (p.prefix_parts == 0)
-        hipLaunchKernelGGL((kv_flash_kernel<FMT, CT, kBothKeys>), grid, block, 0, st, a, f);
+        hipLaunchKernelGGL((kv_flash_kernel<FMT, CT, kBothKeys, W>), grid, block, 0, st, a, f);
       else if (p.prefix_ct == 1)
         hipLaunchKernelGGL((kv_prefix_flash_kernel<FMT, 1, CT < 1 ? CT : 1>), dim3((unsigned)(prefix_blocks + own_blocks)),
                            dim3(256), 0, st, a, f, (int)prefix_blocks, p.own_groups);

@@ -298,9 +298,11 @@ CASES = [  # heads, kv, page, new, own, prefix
     (32, 8, 16, [3], [100], 70), (32, 8, 32, [3, 2], [100, 600], 300), (32, 8, 16, [6, 2], [9, 700], 0),
     (32, 8, 16, [4], [600], 0), (16, 8, 64, [1, 2, 1], [600, 2, 31], 1500), (64, 8, 16, [2], [40], 2100),
     # prefixes long enough to be shared, where those above are read by each sequence
-    (32, 8, 16, [1, 1, 1], [7, 150, 16], 2129), (32, 8, 64, [5, 3, 0, 8], [5, 200, 9, 64], 1033),
-    (5, 5, 16, [17, 16], [17, 90], 1115), (16, 2, 32, [4, 1], [100, 2], 2064), (64, 1, 16, [2], [77], 648),
-    (32, 8, 32, [1], [1], 2048), (32, 8, 16, [1] * 70, list(range(1, 71)), 1200)]
+    (32, 8, 16, [1, 1, 1], [7, 150, 16], 2129), (32, 8, 64, [5, 3, 0, 8], [5, 200, 9, 64], 1633),
+    (5, 5, 16, [17, 16], [17, 90], 1515), (16, 2, 32, [4, 1], [100, 2], 2064), (64, 1, 16, [2], [77], 648),
+    (32, 8, 32, [1], [1], 2048), (32, 8, 16, [1] * 70, list(range(1, 71)), 1200),
+    # two blocks on a CU, with a prefix and without
+    (32, 8, 16, [3] * 40, list(range(3, 43)), 40), (32, 8, 16, [2, 3] * 20, list(range(3, 43)), 0)]
 
 
 @pytest.mark.gpu
@@ -338,7 +340,8 @@ def test_attention_of_many_tiles_a_wave(fmt, heads, kv, page, new, own, prefix, 
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("fmt,new,longest", [(R.F32, 1, 992), (R.INT8, 1, 2016), (R.BF16, 3, 992), (R.FP8, 9, 608)])
+@pytest.mark.parametrize("fmt,new,longest", [(R.F32, 1, 992), (R.INT8, 1, 2016), (R.BF16, 3, 2016), (R.F32, 3, 992),
+                                             (R.INT8, 5, 1504), (R.F32, 5, 736), (R.FP8, 9, 736)])
 def test_attention_around_the_length_that_is_split(fmt, new, longest):
     r = np.random.default_rng(longest)
     pool = Pool(fmt, 8, 32, 140)
